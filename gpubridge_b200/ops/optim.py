@@ -13,7 +13,10 @@ class FlatAdamW:
 
     Arithmetic is ``torch.optim.AdamW``'s.  The step counter lives on the device and is
     advanced by the kernel, so a step can be captured in a CUDA graph.  ``zero_grad`` makes
-    the kernel clear the gradient buffer as it consumes it.
+    the kernel clear the gradient buffer as it consumes it.  ``step(max_norm=...)`` clips the
+    gradients by their global norm on the way: the norm is one launch over the gradient buffer,
+    the factor stays on the device and is taken into the update, so clipped gradients are never
+    written; ``grad_norm`` then holds the norm before clipping (a device tensor).
     """
 
     def __init__(self, flat_param: torch.Tensor, flat_grad: torch.Tensor, lr: float = 1e-3,
@@ -25,8 +28,15 @@ class FlatAdamW:
         self.v = torch.zeros_like(flat_param)
         self.state = torch.zeros(4, dtype=torch.float32, device=flat_param.device)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.grad_norm: torch.Tensor | None = None
 
-    def step(self, grad_scale: float = 1.0, zero_grad: bool = True) -> None:
+    def step(self, grad_scale: float = 1.0, zero_grad: bool = True,
+             max_norm: float | None = None) -> None:
+        """One update of every element.  ``max_norm`` clips the gradients (times ``grad_scale``)
+        to this global 2-norm first, as ``torch.nn.utils.clip_grad_norm_`` does."""
+        if max_norm is not None:
+            self._clipped_step(max_norm, grad_scale, zero_grad)
+            return
         self.step_span(0, self.p.numel(), last=True, grad_scale=grad_scale, zero_grad=zero_grad)
 
     def step_span(self, lo: int, hi: int, last: bool, grad_scale: float = 1.0,
@@ -46,6 +56,26 @@ class FlatAdamW:
             self.betas[1], self.eps, self.weight_decay, grad_scale, int(zero_grad), int(last),
             int(max_blocks), _lib.stream_ptr(self.p.device))
         _lib.check(code, "gb_adamw_span")
+        launches += 1
+
+    def _clipped_step(self, max_norm: float, grad_scale: float, zero_grad: bool) -> None:
+        global launches
+        from gpubridge_b200.ops import grad_clip
+        max_norm = grad_clip._max_norm(max_norm)
+        if self.p.device.type != "cuda":
+            self.grad_norm = grad_clip._cpu_norm([self.g], False, grad_scale)
+            coef = max_norm / (float(self.grad_norm) + 1e-6)
+            self._reference_step(grad_scale * (1.0 if coef > 1.0 else coef), zero_grad)   # a NaN stays one
+            return
+        result = grad_clip._gpu_norm([self.g], self.g.device, False, max_norm, grad_scale)
+        self.grad_norm = result[0]
+        with torch.cuda.device(self.p.device):
+            code = grad_clip._declare(_lib.lib()).gb_adamw_clipped(
+                self.p.data_ptr(), self.g.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
+                self.p.numel(), self.state.data_ptr(), self.lr, self.betas[0], self.betas[1], self.eps,
+                self.weight_decay, grad_scale, result.data_ptr() + 4, int(zero_grad),
+                _lib.stream_ptr(self.p.device))
+        _lib.check(code, "gb_adamw_clipped")
         launches += 1
 
     def _reference_step(self, grad_scale: float, zero_grad: bool, lo: int = 0, hi: int | None = None,

@@ -7,6 +7,7 @@ all-gather GEMM - and keep everything else replicated and in sync.
     ...
     loss.backward()
     sync.average_gradients()                            # one flat all-reduce (AVG) for the rest
+    sync.clip_gradients(1.0)                            # optional: by the norm over all ranks' shards
     optimizer.step()
 
 What FSDP2 does with hooks around every module - all-gather the parameters, run the module,
@@ -53,7 +54,8 @@ class ReplicatedSync:
     """Averages, over the group, the gradients of the parameters that stayed whole."""
 
     def __init__(self, model: nn.Module, topology: Topology | None) -> None:
-        sharded = {id(m.weight) for m in model.modules() if isinstance(m, ShardedLinear)}
+        self.sharded = [m.weight for m in model.modules() if isinstance(m, ShardedLinear)]
+        sharded = {id(w) for w in self.sharded}
         self.topology = topology
         self.params = [p for p in model.parameters() if p.requires_grad and id(p) not in sharded]
         self.numel = sum(p.numel() for p in self.params)
@@ -79,6 +81,22 @@ class ReplicatedSync:
             if p.grad is not None:
                 p.grad.copy_(flat[offset:offset + p.numel()].view_as(p.grad))
             offset += p.numel()
+
+    def clip_gradients(self, max_norm: float) -> torch.Tensor:
+        """Clip every gradient, in place, by the 2-norm of the whole model's: the sharded weights'
+        squares are summed over the group, the replicated parameters (whose gradients are the same
+        everywhere after :meth:`average_gradients`) count once.  Collective.  Returns the norm
+        before clipping; every rank gets the same."""
+        from gpubridge_b200.ops.grad_clip import clip_grads_with_norm_, grad_norm
+        shards = [w.grad for w in self.sharded if w.grad is not None]
+        rest = [p.grad for p in self.params if p.grad is not None]
+        device = (self.sharded + self.params)[0].device
+        square = grad_norm(shards).to(device).double().square()
+        if self.topology is not None and self.topology.world_size > 1:
+            collectives.all_reduce(square, ReduceOp.SUM, _topology=self.topology)
+        norm = (square + grad_norm(rest).to(device).double().square()).sqrt().float()
+        clip_grads_with_norm_(self.sharded + self.params, max_norm, norm)
+        return norm
 
     def memory(self, model: nn.Module) -> dict[str, int]:
         """Bytes of parameters this rank holds: sharded rows, replicated rest."""

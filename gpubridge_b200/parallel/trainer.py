@@ -55,6 +55,10 @@ class DataParallelTrainer:
             for after backward.  The arithmetic and its result are those of one optimizer
             call after backward.  ``GPUBRIDGE_OPTIMIZER_IN_BACKWARD``: ``1``, ``0``, or unset =
             on a team of two or more only (alone it costs more than it hides).
+        max_grad_norm: clip the averaged gradients to this global 2-norm in the optimizer step;
+            ``grad_norm`` then holds the norm before clipping (a device tensor).  The norm needs
+            every gradient, so the update runs after backward: with
+            ``optimizer_in_backward=True`` it is refused, with ``None`` it decides.
     """
 
     def __init__(self, model: nn.Module, loss_fn, *, topology: Topology | None = None,
@@ -63,9 +67,18 @@ class DataParallelTrainer:
                  autocast: torch.dtype | None = torch.bfloat16, graph: bool = False,
                  graph_warmup: int = 3, overlap_blocks: int | None = None,
                  unit_grad: bool = True, exchange: bool = True,
-                 optimizer_in_backward: bool | None = None) -> None:
+                 optimizer_in_backward: bool | None = None,
+                 max_grad_norm: float | None = None) -> None:
         self.model, self.loss_fn = model, loss_fn
         import os
+        if max_grad_norm is not None:
+            if optimizer_in_backward:
+                raise ValueError("max_grad_norm needs every gradient before the first update: "
+                                 "it does not go with optimizer_in_backward=True")
+            if not float(max_grad_norm) >= 0.0:
+                raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+            optimizer_in_backward = False
+        self.max_grad_norm = max_grad_norm
         self.overlap_blocks = overlap_blocks or int(os.environ.get("GPUBRIDGE_OVERLAP_BLOCKS", "0"))
         self._in_backward_wanted = optimizer_in_backward
         # grid of an update that runs beside backward (the last bucket's takes what it wants)
@@ -203,8 +216,8 @@ class DataParallelTrainer:
     # -- the step --------------------------------------------------------------------------------
     def _own_kernels(self) -> int:
         """Launches of this library's kernels so far (every op module keeps a counter)."""
-        from gpubridge_b200.ops import layernorm, optim, xent
-        total = layernorm.launches + optim.launches + xent.launches
+        from gpubridge_b200.ops import grad_clip, layernorm, optim, xent
+        total = layernorm.launches + optim.launches + xent.launches + grad_clip.launches
         if self.fabric is not None:
             total += self.fabric.launches
         return total
@@ -231,7 +244,7 @@ class DataParallelTrainer:
             if self.world > 1 and self.fabric is not None:
                 torch.cuda.current_stream(self.device).wait_stream(self.fabric.comm_stream)
         if not self.optimizer_in_backward:
-            self.optimizer.step(zero_grad=True)
+            self.optimizer.step(zero_grad=True, max_norm=self.max_grad_norm)
         elif self._opt_stream is not None:
             torch.cuda.current_stream(self.device).wait_stream(self._opt_stream)
         self.launches += self._own_kernels() - own_before
@@ -272,6 +285,11 @@ class DataParallelTrainer:
             self._static_loss = self._step_body(self._static_batch)
         self._launches_per_step = self.launches - before
         self.launches = before
+
+    @property
+    def grad_norm(self) -> torch.Tensor | None:
+        """Norm of the averaged gradients of the last step, before clipping (``max_grad_norm``)."""
+        return self.optimizer.grad_norm
 
     def check(self) -> None:
         """Raise if a device-side wait of a collective ran out."""
