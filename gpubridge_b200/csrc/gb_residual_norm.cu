@@ -13,10 +13,11 @@
 //   norm'(g; x^, r) = r * (g w - mean(g w x^) x^ [- mean(g w)])
 //
 // Bound by memory: forward reads residual and update and writes stream and normed, backward reads
-// both gradients, the stream and the update and writes two gradients.  A block owns a row, its
-// values stay in registers between the reductions, and it walks several rows so that the
-// gradients of the parameters, sums over all rows, are gathered in registers; each block leaves
-// its partial sums and a second launch adds them in index order.
+// both gradients, the stream and the update and writes two gradients.  A block owns a row, eight
+// columns a thread; their values stay in registers between the reductions while the next rows are
+// already on their way to shared memory.  A block walks several rows, so that the gradients of the
+// parameters, sums over all rows, are gathered in registers; it leaves its partial sums and a
+// second launch adds them in index order.
 #include "gb_vec.cuh"
 
 namespace {
@@ -34,7 +35,7 @@ struct JoinArgs {
     float* part;                       // [workers][sums][d]
     float* gate_part;                  // [workers + groups - 1][d]
     long long rows, group_rows;        // rows of one gate group
-    int d, layer, param_code, gate_code, next;
+    int d, layer, param_code, gate_code, next, stages;
     float scale, eps;
 };
 
@@ -58,6 +59,18 @@ struct Reducer {
         for (int w = 1; w < warps; ++w) { total.x += b[w].x; total.y += b[w].y; }
         return total;
     }
+    __device__ float sum(float v) {
+        v = gb_warp_sum(v);
+        const int warps = blockDim.x >> 5;
+        if (warps == 1) return v;
+        float* b = reinterpret_cast<float*>(buffer + parity * MAX_WARPS);
+        parity ^= 1;
+        if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
+        __syncthreads();
+        float total = b[0];
+        for (int w = 1; w < warps; ++w) total += b[w];
+        return total;
+    }
 };
 
 // A thread's place in a row: vector k of NV starts at column (k * blockDim.x + threadIdx.x) * VEC.
@@ -73,31 +86,19 @@ struct Lane {
         }
     }
     template <typename T>
-    __device__ void load(const T* row, float (&v)[NV][VEC]) const {
-        if constexpr (VEC == 8) {
-            Raw8<T> raw[NV];
-            #pragma unroll
-            for (int k = 0; k < NV; ++k) if (ok[k]) raw[k].load(row + col[k]);
-            #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                if (ok[k]) raw[k].get(v[k]);
-                else {
-                    #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
-                }
-            }
-        } else {
-            #pragma unroll
-            for (int k = 0; k < NV; ++k) v[k][0] = ok[k] ? gb_up(row[col[k]]) : 0.0f;
-        }
-    }
-    template <typename T>
     __device__ void store(T* row, const float (&v)[NV][VEC]) const {
         #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (!ok[k]) continue;
             if constexpr (VEC == 8) gb_store8(row + col[k], v[k]);
             else row[col[k]] = gb_down<T>(v[k][0]);
+        }
+    }
+    __device__ static void fill(float value, float (&v)[NV][VEC]) {
+        #pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            #pragma unroll
+            for (int j = 0; j < VEC; ++j) v[k][j] = value;
         }
     }
     // a parameter's values in this thread's columns; `otherwise` where there is no such parameter
@@ -112,15 +113,100 @@ struct Lane {
         #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (!ok[k]) continue;
-            #pragma unroll
-            for (int j = 0; j < VEC; ++j) row[col[k] + j] = v[k][j];
+            if constexpr (VEC == 8) gb_store8(row + col[k], v[k]);
+            else row[col[k]] = v[k][0];
         }
     }
 };
 
+// Rows of one tensor on their way to this thread's registers.  Each thread copies the values that
+// it will use itself, STAGES - 1 rows ahead, into its own places in shared memory (cp.async), so
+// the loads of several rows are in flight while a row is reduced, no register holds them and no
+// barrier guards them.  Single values of two bytes cannot be copied so: they are read when used.
+template <typename T, int VEC, int NV>
+struct Feed {
+    static constexpr bool STAGED = VEC == 8 || sizeof(T) == 4;
+    static constexpr int PIECE = VEC == 8 ? 16 : 4;                     // bytes of one copy
+    static constexpr int PIECES = VEC == 8 ? (int)sizeof(T) / 2 : 1;    // copies a vector
+    static constexpr int BYTES = STAGED ? NV * PIECES * PIECE : 0;      // a thread and stage
+    const T* base;
+    long long stride;
+    uint32_t at;                       // shared address of this thread's first piece of stage 0
+    uint32_t stage_bytes;
+    __device__ void place(const void* p, long long row_stride, uint32_t region, uint32_t per_stage) {
+        base = static_cast<const T*>(p);
+        stride = row_stride;
+        at = region + threadIdx.x * PIECE;
+        stage_bytes = per_stage;
+    }
+    __device__ void fetch(const Lane<VEC, NV>& lane, long long row, int stage) const {
+        if constexpr (STAGED) {
+            const T* from = base + row * stride;
+            #pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (!lane.ok[k]) continue;
+                #pragma unroll
+                for (int h = 0; h < PIECES; ++h) {
+                    const uint32_t to = at + stage * stage_bytes + (k * PIECES + h) * blockDim.x * PIECE;
+                    const T* src = from + lane.col[k] + h * (16 / (int)sizeof(T));
+                    if constexpr (PIECE == 16)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(src) : "memory");
+                    else
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(to), "l"(src) : "memory");
+                }
+            }
+        }
+    }
+    __device__ void get(const Lane<VEC, NV>& lane, long long row, int stage, float (&v)[NV][VEC]) const {
+        #pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (!lane.ok[k]) {
+                #pragma unroll
+                for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
+                continue;
+            }
+            if constexpr (VEC == 8) {
+                #pragma unroll
+                for (int h = 0; h < PIECES; ++h) {
+                    const uint32_t from = at + stage * stage_bytes + (k * PIECES + h) * blockDim.x * PIECE;
+                    uint4 q;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(from) : "memory");
+                    if constexpr (sizeof(T) == 4) {
+                        v[k][4 * h] = __uint_as_float(q.x); v[k][4 * h + 1] = __uint_as_float(q.y);
+                        v[k][4 * h + 2] = __uint_as_float(q.z); v[k][4 * h + 3] = __uint_as_float(q.w);
+                    } else {
+                        Raw8<T> raw;
+                        raw.q = q;
+                        raw.get(v[k]);
+                    }
+                }
+            } else if constexpr (STAGED) {
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[k][0])
+                             : "r"(at + stage * stage_bytes + k * blockDim.x * PIECE) : "memory");
+            } else {
+                v[k][0] = gb_up(base[row * stride + lane.col[k]]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ void feed_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// waits until at most `ahead` of the groups this thread committed are under way
+__device__ __forceinline__ void feed_wait(int ahead) {
+    switch (ahead) {
+        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    }
+}
+constexpr int MAX_STAGES = 4;
+
 __device__ __forceinline__ size_t param_bytes(int code) { return code == GB_F32 ? 4 : 2; }
 
-// Mean (0 for rms) and 1 / deviation of a row.
+// Mean (0 for rms) and 1 / deviation of a row.  The variance is that of the centred values, which
+// are at hand: a second reduction instead of a difference of large numbers.
 template <int VEC, int NV>
 __device__ float2 row_stats(const Lane<VEC, NV>& lane, const float (&v)[NV][VEC], int d, int layer,
                             float eps, Reducer& reduce) {
@@ -133,7 +219,7 @@ __device__ float2 row_stats(const Lane<VEC, NV>& lane, const float (&v)[NV][VEC]
             #pragma unroll
             for (int j = 0; j < VEC; ++j) s += v[k][j];
         }
-        mean = reduce.sum(make_float2(s, 0.0f)).x * inv;
+        mean = reduce.sum(s) * inv;
     }
     float q = 0.0f;
     #pragma unroll
@@ -144,34 +230,67 @@ __device__ float2 row_stats(const Lane<VEC, NV>& lane, const float (&v)[NV][VEC]
             q += c * c;
         }
     }
-    const float var = reduce.sum(make_float2(q, 0.0f)).x * inv;
+    const float var = reduce.sum(q) * inv;
     return make_float2(mean, 1.0f / sqrtf(var + eps));
 }
+
+// The gate's values for a row; they are read again where a row begins another group.
+template <int VEC, int NV>
+struct Gate {
+    float v[NV][VEC];
+    long long group = -1, left = 0;    // rows until the next group
+    __device__ Gate() { Lane<VEC, NV>::fill(1.0f, v); }
+    // true where the row begins a group other than the last one's
+    __device__ bool move(const JoinArgs& a, const Lane<VEC, NV>& lane, long long row, long long step) {
+        left -= step;
+        if (left > 0 && group >= 0) return false;
+        const long long mine = row / a.group_rows;
+        left = (mine + 1) * a.group_rows - row;
+        if (mine == group) return false;
+        group = mine;
+        lane.param(static_cast<const char*>(a.gate) + group * a.d * param_bytes(a.gate_code), a.gate_code, 1.0f, v);
+        return true;
+    }
+};
+
+extern __shared__ __align__(16) char join_shared[];
 
 template <typename TS, typename TU, typename TY, int VEC, int NV>
 __global__ void __launch_bounds__(MAX_THREADS) join_fwd_kernel(const JoinArgs a) {
     __shared__ float2 buffer[2 * MAX_WARPS];
     Reducer reduce{buffer};
     const Lane<VEC, NV> lane(a.d);
-    float w[NV][VEC], b[NV][VEC], pw[NV][VEC], pb[NV][VEC], gate[NV][VEC];
+    Feed<TS, VEC, NV> from_residual;
+    Feed<TU, VEC, NV> from_update;
+    constexpr int BYTES = Feed<TS, VEC, NV>::BYTES + Feed<TU, VEC, NV>::BYTES;
+    const uint32_t shared = (uint32_t)__cvta_generic_to_shared(join_shared), per_stage = BYTES * blockDim.x;
+    from_residual.place(a.residual, a.residual_stride, shared, per_stage);
+    from_update.place(a.update, a.update_stride, shared + Feed<TS, VEC, NV>::BYTES * blockDim.x, per_stage);
+    const long long step = gridDim.x;
+    auto fetch = [&](long long row, int stage) {
+        if (row < a.rows) {
+            from_residual.fetch(lane, row, stage);
+            from_update.fetch(lane, row, stage);
+        }
+        feed_commit();
+    };
+    for (int i = 0; i < a.stages - 1; ++i) fetch(blockIdx.x + i * step, i);
+    float w[NV][VEC], b[NV][VEC], pw[NV][VEC], pb[NV][VEC];
     lane.param(a.weight, a.param_code, 1.0f, w);
     lane.param(a.bias, a.param_code, 0.0f, b);
     lane.param(a.post_weight, a.param_code, 1.0f, pw);
     lane.param(a.post_bias, a.param_code, 0.0f, pb);
-    lane.param(nullptr, 0, 1.0f, gate);
-    long long group = -1;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    Gate<VEC, NV> gate;
+    int stage = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += step) {
+        const int ahead = stage == 0 ? a.stages - 1 : stage - 1;
+        fetch(row + (a.stages - 1) * step, ahead);
+        feed_wait(a.stages - 1);
         float u[NV][VEC], r[NV][VEC];
-        lane.load(static_cast<const TU*>(a.update) + row * a.update_stride, u);
-        lane.load(static_cast<const TS*>(a.residual) + row * a.residual_stride, r);
-        if (a.gate) {
-            const long long mine = row / a.group_rows;
-            if (mine != group) {
-                group = mine;
-                lane.param(static_cast<const char*>(a.gate) + group * a.d * param_bytes(a.gate_code),
-                           a.gate_code, 1.0f, gate);
-            }
-        }
+        from_update.get(lane, row, stage, u);
+        from_residual.get(lane, row, stage, r);
+        stage = stage + 1 == a.stages ? 0 : stage + 1;
+        if (a.gate) gate.move(a, lane, row, step);
         float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
         if (a.post_weight) {
             const float2 s = row_stats(lane, u, a.d, a.layer, a.eps, reduce);
@@ -187,7 +306,7 @@ __global__ void __launch_bounds__(MAX_THREADS) join_fwd_kernel(const JoinArgs a)
             #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 // the norm that follows is that of the stream as it is stored
-                r[k][j] = gb_up(gb_down<TS>(fmaf(a.scale * gate[k][j], u[k][j], r[k][j])));
+                r[k][j] = gb_up(gb_down<TS>(fmaf(a.scale * gate.v[k][j], u[k][j], r[k][j])));
                 if (!lane.ok[k]) r[k][j] = 0.0f;
             }
         }
@@ -227,7 +346,8 @@ __device__ void norm_backward(const Lane<VEC, NV>& lane, float (&g)[NV][VEC], co
             s.y += g[k][j];
         }
     }
-    s = reduce.sum(s);
+    if (layer) s = reduce.sum(s);
+    else s.x = reduce.sum(s.x);
     const float inv = 1.0f / (float)d, m1 = s.x * inv, m0 = layer ? s.y * inv : 0.0f;
     #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -240,46 +360,75 @@ __device__ void norm_backward(const Lane<VEC, NV>& lane, float (&g)[NV][VEC], co
 // One block is one worker.  part[worker] holds, one behind the other, the sums of d_weight,
 // d_bias, d_post_weight, d_post_bias that exist.  Worker c and gate group g meet in slot c + g of
 // gate_part: along the rows one of the two grows by one at a time, so no two pairs share a slot.
-template <typename TS, typename TU, typename TY, int VEC, int NV>
+// NEXT: the following norm's gradient takes part; OWN: the update has a norm or a gate of its own.
+template <typename TS, typename TU, typename TY, int VEC, int NV, bool NEXT, bool OWN>
 __global__ void __launch_bounds__(MAX_THREADS) join_bwd_kernel(const JoinArgs a) {
     __shared__ float2 buffer[2 * MAX_WARPS];
     Reducer reduce{buffer};
     const Lane<VEC, NV> lane(a.d);
-    float w[NV][VEC], pw[NV][VEC], pb[NV][VEC], gate[NV][VEC];
+    using FS = Feed<TS, VEC, NV>;
+    using FU = Feed<TU, VEC, NV>;
+    using FY = Feed<TY, VEC, NV>;
+    FS from_grad, from_stream;
+    FU from_update;
+    FY from_normed;
+    constexpr int BYTES = FS::BYTES + (NEXT ? FS::BYTES + FY::BYTES : 0) + (OWN ? FU::BYTES : 0);
+    const uint32_t per_stage = BYTES * blockDim.x;
+    uint32_t region = (uint32_t)__cvta_generic_to_shared(join_shared);
+    from_grad.place(a.d_stream, a.d, region, per_stage);
+    region += FS::BYTES * blockDim.x;
+    if (NEXT) {
+        from_stream.place(a.stream, a.d, region, per_stage);
+        region += FS::BYTES * blockDim.x;
+        from_normed.place(a.d_normed, a.d, region, per_stage);
+        region += FY::BYTES * blockDim.x;
+    }
+    if (OWN) from_update.place(a.update, a.update_stride, region, per_stage);
+    const long long worker = blockIdx.x;
+    const long long lo = first_row(worker, a.rows, gridDim.x), hi = first_row(worker + 1, a.rows, gridDim.x);
+    auto fetch = [&](long long row, int stage) {
+        if (row < hi) {
+            if (a.d_stream) from_grad.fetch(lane, row, stage);
+            if (NEXT) {
+                from_stream.fetch(lane, row, stage);
+                from_normed.fetch(lane, row, stage);
+            }
+            if (OWN) from_update.fetch(lane, row, stage);
+        }
+        feed_commit();
+    };
+    for (int i = 0; i < a.stages - 1; ++i) fetch(lo + i, i);
+    float w[NV][VEC], pw[NV][VEC], pb[NV][VEC];
     float dw[NV][VEC], db[NV][VEC], dpw[NV][VEC], dpb[NV][VEC], dg[NV][VEC];
     lane.param(a.weight, a.param_code, 1.0f, w);
     lane.param(a.post_weight, a.param_code, 1.0f, pw);
     lane.param(a.post_bias, a.param_code, 0.0f, pb);
-    lane.param(nullptr, 0, 1.0f, gate);
-    lane.param(nullptr, 0, 0.0f, dw);
-    lane.param(nullptr, 0, 0.0f, db);
-    lane.param(nullptr, 0, 0.0f, dpw);
-    lane.param(nullptr, 0, 0.0f, dpb);
-    lane.param(nullptr, 0, 0.0f, dg);
-    const bool needs_update = a.post_weight || a.gate;
-    const long long worker = blockIdx.x;
-    const long long lo = first_row(worker, a.rows, gridDim.x), hi = first_row(worker + 1, a.rows, gridDim.x);
-    long long group = -1;
+    Gate<VEC, NV> gate;
+    lane.fill(0.0f, dw);
+    lane.fill(0.0f, db);
+    lane.fill(0.0f, dpw);
+    lane.fill(0.0f, dpb);
+    lane.fill(0.0f, dg);
+    int stage = 0;
     for (long long row = lo; row < hi; ++row) {
-        if (a.gate) {
-            const long long mine = row / a.group_rows;
-            if (mine != group) {
-                if (group >= 0) lane.sums(a.gate_part + (worker + group) * a.d, dg);
-                group = mine;
-                lane.param(nullptr, 0, 0.0f, dg);
-                lane.param(static_cast<const char*>(a.gate) + group * a.d * param_bytes(a.gate_code),
-                           a.gate_code, 1.0f, gate);
+        const int ahead = stage == 0 ? a.stages - 1 : stage - 1;
+        fetch(row + a.stages - 1, ahead);
+        const float4 st = a.stats[row];
+        if (OWN && a.gate) {
+            const long long before = gate.group;
+            if (gate.move(a, lane, row, 1) && before >= 0) {
+                lane.sums(a.gate_part + (worker + before) * a.d, dg);
+                lane.fill(0.0f, dg);
             }
         }
-        float dr[NV][VEC], u[NV][VEC];
-        const float4 st = a.stats[row];
-        if (a.d_stream) lane.load(static_cast<const TS*>(a.d_stream) + row * a.d, dr);
-        else lane.param(nullptr, 0, 0.0f, dr);
-        if (needs_update) lane.load(static_cast<const TU*>(a.update) + row * a.update_stride, u);
-        if (a.d_normed) {
+        feed_wait(a.stages - 1);
+        float dr[NV][VEC];
+        if (a.d_stream) from_grad.get(lane, row, stage, dr);
+        else lane.fill(0.0f, dr);
+        if (NEXT) {
             float g[NV][VEC], hat[NV][VEC];
-            lane.load(static_cast<const TY*>(a.d_normed) + row * a.d, g);
-            lane.load(static_cast<const TS*>(a.stream) + row * a.d, hat);
+            from_normed.get(lane, row, stage, g);
+            from_stream.get(lane, row, stage, hat);
             #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 #pragma unroll
@@ -303,14 +452,16 @@ __global__ void __launch_bounds__(MAX_THREADS) join_bwd_kernel(const JoinArgs a)
             #pragma unroll
             for (int j = 0; j < VEC; ++j) dr[k][j] *= a.scale;
         }
-        if (needs_update) {
+        if (OWN) {
+            float u[NV][VEC];
+            from_update.get(lane, row, stage, u);
             #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     u[k][j] = (u[k][j] - st.x) * st.y;            // the update itself without a post norm
                     dg[k][j] += dr[k][j] * (u[k][j] * pw[k][j] + pb[k][j]);
-                    dr[k][j] *= gate[k][j];
+                    dr[k][j] *= gate.v[k][j];
                     dpw[k][j] += dr[k][j] * u[k][j];
                     dpb[k][j] += dr[k][j];
                     dr[k][j] *= pw[k][j];
@@ -319,14 +470,15 @@ __global__ void __launch_bounds__(MAX_THREADS) join_bwd_kernel(const JoinArgs a)
             if (a.post_weight) norm_backward(lane, dr, u, st.y, a.d, a.layer, reduce);
         }
         lane.store(static_cast<TU*>(a.d_update) + row * a.d, dr);
+        stage = stage + 1 == a.stages ? 0 : stage + 1;
     }
-    if (a.gate && group >= 0) lane.sums(a.gate_part + (worker + group) * a.d, dg);
-    const int sums = (a.d_normed ? (a.bias ? 2 : 1) : 0) + (a.post_weight ? (a.post_bias ? 2 : 1) : 0);
+    if (OWN && a.gate && gate.group >= 0) lane.sums(a.gate_part + (worker + gate.group) * a.d, dg);
+    const int sums = (NEXT ? (a.bias ? 2 : 1) : 0) + (a.post_weight ? (a.post_bias ? 2 : 1) : 0);
     float* mine = a.part + worker * sums * a.d;
-    if (a.d_normed) { lane.sums(mine, dw); mine += a.d; }
-    if (a.d_normed && a.bias) { lane.sums(mine, db); mine += a.d; }
-    if (a.post_weight) { lane.sums(mine, dpw); mine += a.d; }
-    if (a.post_weight && a.post_bias) lane.sums(mine, dpb);
+    if (NEXT) { lane.sums(mine, dw); mine += a.d; }
+    if (NEXT && a.bias) { lane.sums(mine, db); mine += a.d; }
+    if (OWN && a.post_weight) { lane.sums(mine, dpw); mine += a.d; }
+    if (OWN && a.post_weight && a.post_bias) lane.sums(mine, dpb);
 }
 
 struct SumArgs {
@@ -371,46 +523,69 @@ __global__ void __launch_bounds__(32 * SLICES) join_sum_kernel(const SumArgs a) 
 
 constexpr int MAX_WIDTH = 8192;
 
-// Threads of a block for rows of d values in vectors of vec.
-int threads_for(int d, int vec) {
-    int t = (d + vec - 1) / vec;
-    t = (t + 31) / 32 * 32;
-    return t < MAX_THREADS ? t : MAX_THREADS;
+// Threads of a block for rows of d values in vectors of vec, and its rounds of vectors: a single
+// round of eight columns a thread up to 4096 columns, two from there on; single values in up to
+// four rounds of 256 threads, then sixteen of 512.
+struct Shape { int threads, rounds; };
+Shape shape_of(int d, int vec) {
+    const int vectors = (d + vec - 1) / vec, most = vec == 8 || vectors > 1024 ? MAX_THREADS : 256;
+    int t = (vectors + 31) / 32 * 32;
+    if (t > most) t = most;
+    return Shape{t, (vectors + t - 1) / t};
+}
+
+// Blocks an SM holds at the 128 registers that 512 threads may have; each leaves a row of partial
+// sums, so there are no more than fill the SMs.
+int blocks_per_sm(int threads) {
+    const int n = 512 / threads;
+    return n < 1 ? 1 : n > 8 ? 8 : n;
 }
 
 int workers_for(long long rows, int threads) {
-    // enough blocks to fill the SMs at the registers these kernels take, and no more: each leaves
-    // a row of partial sums
-    int per_sm = 512 / threads;
-    if (per_sm < 1) per_sm = 1;
-    if (per_sm > 8) per_sm = 8;
-    const long long most = 148LL * per_sm;
+    const long long most = 148LL * blocks_per_sm(threads);
     return (int)(rows < most ? rows : most);
+}
+
+// Stages that fit beside one another in an SM's 227 KB.
+int stages_for(int bytes_per_stage, int blocks) {
+    int n = bytes_per_stage ? (int)((220 << 10) / blocks / bytes_per_stage) : MAX_STAGES;
+    return n < 1 ? 1 : n > MAX_STAGES ? MAX_STAGES : n;
+}
+
+template <typename K>
+int start(K kernel, int grid, int threads, int bytes_per_stage, int blocks, JoinArgs a, cudaStream_t s) {
+    a.stages = stages_for(bytes_per_stage, blocks);
+    const int shared = a.stages * bytes_per_stage;
+    if (shared > (40 << 10)) {                       // more than a launch may take unasked, with the static part
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+        if (err != cudaSuccess) return (int)err;
+    }
+    kernel<<<grid, threads, shared, s>>>(a);
+    return (int)cudaGetLastError();
+}
+
+template <typename TS, typename TU, typename TY, int VEC, int NV>
+int launch_shaped(bool forward, int threads, const JoinArgs& a, cudaStream_t s) {
+    constexpr int S = Feed<TS, VEC, NV>::BYTES, U = Feed<TU, VEC, NV>::BYTES, Y = Feed<TY, VEC, NV>::BYTES;
+    const int blocks = blocks_per_sm(threads);
+    const int grid = workers_for(a.rows, threads);
+    if (forward) return start(join_fwd_kernel<TS, TU, TY, VEC, NV>, grid, threads, (S + U) * threads, blocks, a, s);
+    const bool next = a.d_normed, own = a.post_weight || a.gate;
+    if (next && own) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, true, true>, grid, threads, (2 * S + Y + U) * threads, blocks, a, s);
+    if (next) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, true, false>, grid, threads, (2 * S + Y) * threads, blocks, a, s);
+    return start(join_bwd_kernel<TS, TU, TY, VEC, NV, false, true>, grid, threads, (S + U) * threads, blocks, a, s);
 }
 
 template <typename TS, typename TU, typename TY>
 int launch(bool forward, int vec, const JoinArgs& a, cudaStream_t s) {
-    const int t = threads_for(a.d, vec);
-    const int nv = (a.d + t * vec - 1) / (t * vec);
-    long long grid;
-    if (forward) {
-        long long cap = 148LL * (2048 / t < 16 ? 2048 / t : 16);
-        grid = a.rows < cap ? a.rows : cap;
-    } else grid = workers_for(a.rows, t);
-#define GB_JOIN(VEC, NV) (forward ? join_fwd_kernel<TS, TU, TY, VEC, NV><<<(int)grid, t, 0, s>>>(a) \
-                                  : join_bwd_kernel<TS, TU, TY, VEC, NV><<<(int)grid, t, 0, s>>>(a))
+    const Shape shape = shape_of(a.d, vec);
     if (vec == 8) {
-        if (nv <= 1) GB_JOIN(8, 1);
-        else if (nv <= 2) GB_JOIN(8, 2);
-        else return (int)cudaErrorInvalidValue;
-    } else {
-        if (nv <= 1) GB_JOIN(1, 1);
-        else if (nv <= 4) GB_JOIN(1, 4);
-        else if (nv <= 16) GB_JOIN(1, 16);
-        else return (int)cudaErrorInvalidValue;
+        if (shape.rounds == 1) return launch_shaped<TS, TU, TY, 8, 1>(forward, shape.threads, a, s);
+        return launch_shaped<TS, TU, TY, 8, 2>(forward, shape.threads, a, s);
     }
-#undef GB_JOIN
-    return (int)cudaGetLastError();
+    if (shape.rounds <= 1) return launch_shaped<TS, TU, TY, 1, 1>(forward, shape.threads, a, s);
+    if (shape.rounds <= 4) return launch_shaped<TS, TU, TY, 1, 4>(forward, shape.threads, a, s);
+    return launch_shaped<TS, TU, TY, 1, 16>(forward, shape.threads, a, s);
 }
 
 int dispatch(bool forward, int s, int u, int y, int vec, const JoinArgs& a, cudaStream_t stream) {
@@ -449,7 +624,7 @@ extern "C" int gb_residual_norm_fwd(int s, int u, int y, int vec, const void* re
 // Workers (blocks) of a backward call: part holds workers * sums * d floats, gate_part
 // (workers + groups - 1) * d.
 extern "C" int gb_residual_norm_workers(long long rows, int d, int vec) {
-    return workers_for(rows, threads_for(d, vec));
+    return workers_for(rows, shape_of(d, vec).threads);
 }
 
 // The stream, both gradients (either may be null) and the outputs are [rows, d] without gaps;
