@@ -35,47 +35,92 @@ struct JoinArgs {
     float* part;                       // [workers][sums][d]
     float* gate_part;                  // [workers + groups - 1][d]
     long long rows, group_rows;        // rows of one gate group
-    int d, layer, param_code, gate_code, next, stages;
+    int d, layer, param_code, gate_code, next, slots;
     float scale, eps;
 };
 
 constexpr int MAX_THREADS = 512;
 constexpr int MAX_WARPS = MAX_THREADS / 32;
 
-// Sums over the block's threads; the buffers alternate, so one barrier a reduction is enough.
+// Two values in one instruction (sm_100a's packed fp32); each rounds as the single one does.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+          "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Sums of Q values over the block's threads, one barrier a reduction: the buffers alternate.
+// Within a warp the values are exchanged for one another before they are added, so that Q = 1, 2,
+// 4 cost five, five and six shuffles.
 struct Reducer {
-    float2* buffer;                    // [2][MAX_WARPS]
-    int parity = 0;
-    __device__ float2 sum(float2 v) {
-        v.x = gb_warp_sum(v.x);
-        v.y = gb_warp_sum(v.y);
-        const int warps = blockDim.x >> 5;
-        if (warps == 1) return v;
-        float2* b = buffer + parity * MAX_WARPS;
-        parity ^= 1;
-        if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
+    float* buffer;                     // [2][MAX_WARPS][4]
+    int warps, parity;
+    __device__ explicit Reducer(float* b) : buffer(b), warps((int)blockDim.x >> 5), parity(0) {
+        for (int i = threadIdx.x; i < 2 * MAX_WARPS * 4; i += blockDim.x) b[i] = 0.0f;
         __syncthreads();
-        float2 total = b[0];
-        for (int w = 1; w < warps; ++w) { total.x += b[w].x; total.y += b[w].y; }
-        return total;
     }
-    __device__ float sum(float v) {
-        v = gb_warp_sum(v);
-        const int warps = blockDim.x >> 5;
-        if (warps == 1) return v;
-        float* b = reinterpret_cast<float*>(buffer + parity * MAX_WARPS);
+    template <int Q>
+    __device__ void sum(float (&v)[Q]) {
+        static_assert(Q == 1 || Q == 2 || Q == 4, "values of one reduction");
+        const int lane = threadIdx.x & 31;
+        float mine;
+        if constexpr (Q == 4) {
+            const bool upper = lane & 16;
+            float a = upper ? v[2] : v[0], b = upper ? v[3] : v[1];
+            const float sa = upper ? v[0] : v[2], sb = upper ? v[1] : v[3];
+            a += __shfl_xor_sync(0xffffffffu, sa, 16);
+            b += __shfl_xor_sync(0xffffffffu, sb, 16);
+            const bool second = lane & 8;
+            mine = second ? b : a;
+            mine += __shfl_xor_sync(0xffffffffu, second ? a : b, 8);
+        } else if constexpr (Q == 2) {
+            const bool upper = lane & 16;
+            mine = upper ? v[1] : v[0];
+            mine += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[1], 16);
+        } else mine = v[0];
+        #pragma unroll
+        for (int step = Q == 4 ? 4 : Q == 2 ? 8 : 16; step > 0; step >>= 1)
+            mine += __shfl_xor_sync(0xffffffffu, mine, step);
+        float* b = buffer + parity * MAX_WARPS * 4;
         parity ^= 1;
-        if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-        __syncthreads();
-        float total = b[0];
-        for (int w = 1; w < warps; ++w) total += b[w];
-        return total;
+        if (lane % (32 / Q) == 0) b[(threadIdx.x >> 5) * Q + lane / (32 / Q)] = mine;
+        if (warps == 1) __syncwarp(); else __syncthreads();
+        // all partial results, four warps at a time (there are zeros behind the last)
+        const float4* b4 = reinterpret_cast<const float4*>(b);
+        #pragma unroll
+        for (int q = 0; q < Q; ++q) v[q] = 0.0f;
+        for (int w = 0; w < warps; w += 4) {
+            #pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                const float4 f = b4[(w / 4) * Q + i];
+                const float e[4] = {f.x, f.y, f.z, f.w};
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) v[(4 * i + j) % Q] += e[j];
+            }
+        }
     }
 };
 
 // A thread's place in a row: vector k of NV starts at column (k * blockDim.x + threadIdx.x) * VEC.
+// Its values are held in pairs: value e of the thread is that of vector e / VEC.
 template <int VEC, int NV>
 struct Lane {
+    static constexpr int E = VEC * NV, P = (E + 1) / 2;
     int col[NV];
     bool ok[NV];
     __device__ explicit Lane(int d) {
@@ -85,61 +130,61 @@ struct Lane {
             ok[k] = col[k] < d;                     // d is a multiple of VEC
         }
     }
+    __device__ static float& at(float2 (&v)[P], int e) { return e & 1 ? v[e / 2].y : v[e / 2].x; }
+    __device__ static float at(const float2 (&v)[P], int e) { return e & 1 ? v[e / 2].y : v[e / 2].x; }
     template <typename T>
-    __device__ void store(T* row, const float (&v)[NV][VEC]) const {
+    __device__ void store(T* row, const float2 (&v)[P]) const {
         #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (!ok[k]) continue;
-            if constexpr (VEC == 8) gb_store8(row + col[k], v[k]);
-            else row[col[k]] = gb_down<T>(v[k][0]);
+            if constexpr (VEC == 8) {
+                float f[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = at(v, k * 8 + j);
+                gb_store8(row + col[k], f);
+            } else row[col[k]] = gb_down<T>(at(v, k));
         }
     }
-    __device__ static void fill(float value, float (&v)[NV][VEC]) {
+    __device__ static void fill(float value, float2 (&v)[P]) {
         #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[k][j] = value;
-        }
+        for (int i = 0; i < P; ++i) v[i] = both(value);
+    }
+    // 0 in the places of no column
+    __device__ void mask(float2 (&v)[P]) const {
+        #pragma unroll
+        for (int e = 0; e < E; ++e) if (!ok[e / VEC]) at(v, e) = 0.0f;
+        if (E & 1) v[P - 1].y = 0.0f;
     }
     // a parameter's values in this thread's columns; `otherwise` where there is no such parameter
-    __device__ void param(const void* p, int code, float otherwise, float (&v)[NV][VEC]) const {
+    __device__ void param(const void* p, int code, float otherwise, float2 (&v)[P]) const {
+        fill(otherwise, v);
+        if (!p) return;
         #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[k][j] = (p && ok[k]) ? gb_read(p, code, col[k] + j) : otherwise;
-        }
-    }
-    __device__ void sums(float* row, const float (&v)[NV][VEC]) const {
-        #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (!ok[k]) continue;
-            if constexpr (VEC == 8) gb_store8(row + col[k], v[k]);
-            else row[col[k]] = v[k][0];
-        }
+        for (int e = 0; e < E; ++e) if (ok[e / VEC]) at(v, e) = gb_read(p, code, col[e / VEC] + e % VEC);
     }
 };
 
 // Rows of one tensor on their way to this thread's registers.  Each thread copies the values that
-// it will use itself, STAGES - 1 rows ahead, into its own places in shared memory (cp.async), so
-// the loads of several rows are in flight while a row is reduced, no register holds them and no
-// barrier guards them.  Single values of two bytes cannot be copied so: they are read when used.
+// it will use itself into its own places in shared memory (cp.async), as many rows ahead as there
+// are slots, so the loads of several rows are in flight while a row is reduced, no register holds
+// them and no barrier guards them.  Single values of two bytes cannot be copied so: they are read
+// when used.
 template <typename T, int VEC, int NV>
 struct Feed {
     static constexpr bool STAGED = VEC == 8 || sizeof(T) == 4;
     static constexpr int PIECE = VEC == 8 ? 16 : 4;                     // bytes of one copy
     static constexpr int PIECES = VEC == 8 ? (int)sizeof(T) / 2 : 1;    // copies a vector
-    static constexpr int BYTES = STAGED ? NV * PIECES * PIECE : 0;      // a thread and stage
+    static constexpr int BYTES = STAGED ? NV * PIECES * PIECE : 0;      // a thread and slot
+    using L = Lane<VEC, NV>;
     const T* base;
     long long stride;
-    uint32_t at;                       // shared address of this thread's first piece of stage 0
-    uint32_t stage_bytes;
-    __device__ void place(const void* p, long long row_stride, uint32_t region, uint32_t per_stage) {
+    uint32_t at;                       // shared address of this thread's first piece of slot 0
+    __device__ void place(const void* p, long long row_stride, uint32_t region) {
         base = static_cast<const T*>(p);
         stride = row_stride;
         at = region + threadIdx.x * PIECE;
-        stage_bytes = per_stage;
     }
-    __device__ void fetch(const Lane<VEC, NV>& lane, long long row, int stage) const {
+    __device__ void fetch(const L& lane, long long row, uint32_t slot_offset) const {
         if constexpr (STAGED) {
             const T* from = base + row * stride;
             #pragma unroll
@@ -147,7 +192,7 @@ struct Feed {
                 if (!lane.ok[k]) continue;
                 #pragma unroll
                 for (int h = 0; h < PIECES; ++h) {
-                    const uint32_t to = at + stage * stage_bytes + (k * PIECES + h) * blockDim.x * PIECE;
+                    const uint32_t to = at + slot_offset + (k * PIECES + h) * blockDim.x * PIECE;
                     const T* src = from + lane.col[k] + h * (16 / (int)sizeof(T));
                     if constexpr (PIECE == 16)
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(src) : "memory");
@@ -157,173 +202,59 @@ struct Feed {
             }
         }
     }
-    __device__ void get(const Lane<VEC, NV>& lane, long long row, int stage, float (&v)[NV][VEC]) const {
+    __device__ void get(const L& lane, long long row, uint32_t slot_offset, float2 (&v)[L::P]) const {
+        if (L::E & 1) v[L::P - 1].y = 0.0f;
         #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (!lane.ok[k]) {
-                #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
-                continue;
-            }
             if constexpr (VEC == 8) {
-                #pragma unroll
-                for (int h = 0; h < PIECES; ++h) {
-                    const uint32_t from = at + stage * stage_bytes + (k * PIECES + h) * blockDim.x * PIECE;
-                    uint4 q;
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(from) : "memory");
-                    if constexpr (sizeof(T) == 4) {
-                        v[k][4 * h] = __uint_as_float(q.x); v[k][4 * h + 1] = __uint_as_float(q.y);
-                        v[k][4 * h + 2] = __uint_as_float(q.z); v[k][4 * h + 3] = __uint_as_float(q.w);
-                    } else {
-                        Raw8<T> raw;
-                        raw.q = q;
-                        raw.get(v[k]);
+                float f[8] = {};
+                if (lane.ok[k]) {
+                    #pragma unroll
+                    for (int h = 0; h < PIECES; ++h) {
+                        const uint32_t from = at + slot_offset + (k * PIECES + h) * blockDim.x * PIECE;
+                        uint4 q;
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(from) : "memory");
+                        if constexpr (sizeof(T) == 4) {
+                            f[4 * h] = __uint_as_float(q.x); f[4 * h + 1] = __uint_as_float(q.y);
+                            f[4 * h + 2] = __uint_as_float(q.z); f[4 * h + 3] = __uint_as_float(q.w);
+                        } else {
+                            Raw8<T> raw;
+                            raw.q = q;
+                            raw.get(f);
+                        }
                     }
                 }
-            } else if constexpr (STAGED) {
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[k][0])
-                             : "r"(at + stage * stage_bytes + k * blockDim.x * PIECE) : "memory");
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) L::at(v, k * 8 + j) = f[j];
             } else {
-                v[k][0] = gb_up(base[row * stride + lane.col[k]]);
+                float f = 0.0f;
+                if (lane.ok[k]) {
+                    if constexpr (STAGED)
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f)
+                                     : "r"(at + slot_offset + k * blockDim.x * PIECE) : "memory");
+                    else f = gb_up(base[row * stride + lane.col[k]]);
+                }
+                L::at(v, k) = f;
             }
         }
     }
 };
 
 __device__ __forceinline__ void feed_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// waits until at most `ahead` of the groups this thread committed are under way
-__device__ __forceinline__ void feed_wait(int ahead) {
-    switch (ahead) {
+// waits until at most `behind` of the groups this thread committed are under way
+__device__ __forceinline__ void feed_wait(int behind) {
+    switch (behind) {
         case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
         case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
         case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
     }
 }
-constexpr int MAX_STAGES = 4;
-
-__device__ __forceinline__ size_t param_bytes(int code) { return code == GB_F32 ? 4 : 2; }
-
-// Mean (0 for rms) and 1 / deviation of a row.  The variance is that of the centred values, which
-// are at hand: a second reduction instead of a difference of large numbers.
-template <int VEC, int NV>
-__device__ float2 row_stats(const Lane<VEC, NV>& lane, const float (&v)[NV][VEC], int d, int layer,
-                            float eps, Reducer& reduce) {
-    const float inv = 1.0f / (float)d;
-    float mean = 0.0f;
-    if (layer) {
-        float s = 0.0f;
-        #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += v[k][j];
-        }
-        mean = reduce.sum(s) * inv;
-    }
-    float q = 0.0f;
-    #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float c = lane.ok[k] ? v[k][j] - mean : 0.0f;
-            q += c * c;
-        }
-    }
-    const float var = reduce.sum(q) * inv;
-    return make_float2(mean, 1.0f / sqrtf(var + eps));
-}
-
-// The gate's values for a row; they are read again where a row begins another group.
-template <int VEC, int NV>
-struct Gate {
-    float v[NV][VEC];
-    long long group = -1, left = 0;    // rows until the next group
-    __device__ Gate() { Lane<VEC, NV>::fill(1.0f, v); }
-    // true where the row begins a group other than the last one's
-    __device__ bool move(const JoinArgs& a, const Lane<VEC, NV>& lane, long long row, long long step) {
-        left -= step;
-        if (left > 0 && group >= 0) return false;
-        const long long mine = row / a.group_rows;
-        left = (mine + 1) * a.group_rows - row;
-        if (mine == group) return false;
-        group = mine;
-        lane.param(static_cast<const char*>(a.gate) + group * a.d * param_bytes(a.gate_code), a.gate_code, 1.0f, v);
-        return true;
-    }
-};
-
-extern __shared__ __align__(16) char join_shared[];
-
-template <typename TS, typename TU, typename TY, int VEC, int NV>
-__global__ void __launch_bounds__(MAX_THREADS) join_fwd_kernel(const JoinArgs a) {
-    __shared__ float2 buffer[2 * MAX_WARPS];
-    Reducer reduce{buffer};
-    const Lane<VEC, NV> lane(a.d);
-    Feed<TS, VEC, NV> from_residual;
-    Feed<TU, VEC, NV> from_update;
-    constexpr int BYTES = Feed<TS, VEC, NV>::BYTES + Feed<TU, VEC, NV>::BYTES;
-    const uint32_t shared = (uint32_t)__cvta_generic_to_shared(join_shared), per_stage = BYTES * blockDim.x;
-    from_residual.place(a.residual, a.residual_stride, shared, per_stage);
-    from_update.place(a.update, a.update_stride, shared + Feed<TS, VEC, NV>::BYTES * blockDim.x, per_stage);
-    const long long step = gridDim.x;
-    auto fetch = [&](long long row, int stage) {
-        if (row < a.rows) {
-            from_residual.fetch(lane, row, stage);
-            from_update.fetch(lane, row, stage);
-        }
-        feed_commit();
-    };
-    for (int i = 0; i < a.stages - 1; ++i) fetch(blockIdx.x + i * step, i);
-    float w[NV][VEC], b[NV][VEC], pw[NV][VEC], pb[NV][VEC];
-    lane.param(a.weight, a.param_code, 1.0f, w);
-    lane.param(a.bias, a.param_code, 0.0f, b);
-    lane.param(a.post_weight, a.param_code, 1.0f, pw);
-    lane.param(a.post_bias, a.param_code, 0.0f, pb);
-    Gate<VEC, NV> gate;
-    int stage = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += step) {
-        const int ahead = stage == 0 ? a.stages - 1 : stage - 1;
-        fetch(row + (a.stages - 1) * step, ahead);
-        feed_wait(a.stages - 1);
-        float u[NV][VEC], r[NV][VEC];
-        from_update.get(lane, row, stage, u);
-        from_residual.get(lane, row, stage, r);
-        stage = stage + 1 == a.stages ? 0 : stage + 1;
-        if (a.gate) gate.move(a, lane, row, step);
-        float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-        if (a.post_weight) {
-            const float2 s = row_stats(lane, u, a.d, a.layer, a.eps, reduce);
-            st.x = s.x; st.y = s.y;
-            #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                #pragma unroll
-                for (int j = 0; j < VEC; ++j) u[k][j] = (u[k][j] - s.x) * s.y * pw[k][j] + pb[k][j];
-            }
-        }
-        #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                // the norm that follows is that of the stream as it is stored
-                r[k][j] = gb_up(gb_down<TS>(fmaf(a.scale * gate.v[k][j], u[k][j], r[k][j])));
-                if (!lane.ok[k]) r[k][j] = 0.0f;
-            }
-        }
-        lane.store(static_cast<TS*>(a.stream) + row * a.d, r);
-        if (a.next) {
-            const float2 s = row_stats(lane, r, a.d, a.layer, a.eps, reduce);
-            st.z = s.x; st.w = s.y;
-            #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                #pragma unroll
-                for (int j = 0; j < VEC; ++j) r[k][j] = (r[k][j] - s.x) * s.y * w[k][j] + b[k][j];
-            }
-            lane.store(static_cast<TY*>(a.normed) + row * a.d, r);
-        }
-        if (a.stats && threadIdx.x == 0) a.stats[row] = st;
-    }
-}
+constexpr int MAX_SLOTS = 8;
 
 // Worker c owns the rows [first_row(c), first_row(c + 1)); owner_of is its inverse.
 __host__ __device__ __forceinline__ long long first_row(long long c, long long rows, long long workers) {
@@ -333,39 +264,222 @@ __host__ __device__ __forceinline__ long long owner_of(long long row, long long 
     return ((row + 1) * workers - 1) / rows;
 }
 
-// r * (g - mean(g x^) x^ [- mean(g)]) over a row, g given in place.
-template <int VEC, int NV>
-__device__ void norm_backward(const Lane<VEC, NV>& lane, float (&g)[NV][VEC], const float (&hat)[NV][VEC],
-                              float rstd, int d, int layer, Reducer& reduce) {
-    float2 s = make_float2(0.0f, 0.0f);
-    #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            s.x += g[k][j] * hat[k][j];
-            s.y += g[k][j];
+// A worker's walk over its rows: up to R at a time, all of one gate group, with the rows behind
+// them under way.  One group of copies a row, in the rows' order, so a wait for all but the last
+// slots - R groups is a wait for the rows at hand.
+template <int R>
+struct Walk {
+    long long row, hi, fetched, group, group_end, group_rows;
+    int slots, slot, count, fetch_slot;
+    bool gated;
+    __device__ Walk(const JoinArgs& a)
+        : row(first_row(blockIdx.x, a.rows, gridDim.x)), hi(first_row(blockIdx.x + 1LL, a.rows, gridDim.x)),
+          fetched(row), group(-1), group_end(hi), group_rows(a.group_rows), slots(a.slots), slot(0), count(0),
+          fetch_slot(0), gated(a.gate != nullptr) {}
+    template <typename F>
+    __device__ void ahead(int n, F fetch) {         // the next n rows' copies; empty groups behind the last row
+        for (int i = 0; i < n; ++i) {
+            if (fetched < hi) fetch(fetched, fetch_slot);
+            feed_commit();
+            ++fetched;
+            fetch_slot = fetch_slot + 1 == slots ? 0 : fetch_slot + 1;
         }
     }
-    if (layer) s = reduce.sum(s);
-    else s.x = reduce.sum(s.x);
-    const float inv = 1.0f / (float)d, m1 = s.x * inv, m0 = layer ? s.y * inv : 0.0f;
-    #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            g[k][j] = lane.ok[k] ? rstd * (g[k][j] - m0 - hat[k][j] * m1) : 0.0f;
+    // the rows at hand are row .. row + count - 1; true where they begin another group
+    __device__ bool next() {
+        bool fresh = false;
+        if (gated && (group < 0 || row >= group_end)) {
+            group = row / group_rows;
+            group_end = (group + 1) * group_rows;
+            fresh = true;
+        }
+        const long long end = gated && group_end < hi ? group_end : hi;
+        count = end - row < R ? (int)(end - row) : R;
+        return fresh;
     }
+    __device__ int slot_of(int i) const { const int s = slot + i; return s >= slots ? s - slots : s; }
+    __device__ void done() { row += count; slot = slot_of(count); }
+};
+
+__device__ __forceinline__ size_t param_bytes(int code) { return code == GB_F32 ? 4 : 2; }
+
+// Mean (0 for rms) and 1 / deviation of R rows.  The variance is that of the centred values, which
+// are at hand: a second reduction instead of a difference of large numbers.
+template <bool LAYER, int VEC, int NV, int R>
+__device__ void row_stats(const Lane<VEC, NV>& lane, float2 (&v)[R][Lane<VEC, NV>::P], float inv_d, float eps,
+                          Reducer& reduce, float (&mean)[R], float (&rstd)[R]) {
+    constexpr int P = Lane<VEC, NV>::P;
+    if constexpr (LAYER) {
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float2 s = v[i][0];
+            #pragma unroll
+            for (int e = 1; e < P; ++e) s = add2(s, v[i][e]);
+            mean[i] = s.x + s.y;
+        }
+        reduce.sum(mean);
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            mean[i] *= inv_d;
+            #pragma unroll
+            for (int e = 0; e < P; ++e) v[i][e] = add2(v[i][e], both(-mean[i]));
+            lane.mask(v[i]);
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+        float2 q = mul2(v[i][0], v[i][0]);
+        #pragma unroll
+        for (int e = 1; e < P; ++e) q = fma2(v[i][e], v[i][e], q);
+        rstd[i] = q.x + q.y;
+    }
+    reduce.sum(rstd);
+    #pragma unroll
+    for (int i = 0; i < R; ++i) rstd[i] = 1.0f / sqrtf(rstd[i] * inv_d + eps);
+}
+
+extern __shared__ __align__(16) char join_shared[];
+
+// FULL: layer norms, or any bias; otherwise rms norms without.
+template <typename TS, typename TU, typename TY, int VEC, int NV, int R, bool FULL>
+__global__ void __launch_bounds__(MAX_THREADS) join_fwd_kernel(const JoinArgs a) {
+    __shared__ __align__(16) float buffer[2 * MAX_WARPS * 4];
+    using L = Lane<VEC, NV>;
+    constexpr int P = L::P;
+    const L lane(a.d);
+    Feed<TS, VEC, NV> from_residual;
+    Feed<TU, VEC, NV> from_update;
+    constexpr int BYTES = Feed<TS, VEC, NV>::BYTES + Feed<TU, VEC, NV>::BYTES;
+    const uint32_t shared = (uint32_t)__cvta_generic_to_shared(join_shared), per_slot = BYTES * blockDim.x;
+    from_residual.place(a.residual, a.residual_stride, shared);
+    from_update.place(a.update, a.update_stride, shared + Feed<TS, VEC, NV>::BYTES * blockDim.x);
+    Walk<R> walk(a);
+    auto fetch = [&](long long row, int slot) {
+        from_residual.fetch(lane, row, slot * per_slot);
+        from_update.fetch(lane, row, slot * per_slot);
+    };
+    walk.ahead(walk.slots, fetch);
+    Reducer reduce(buffer);
+    const float inv_d = 1.0f / (float)a.d;
+    float2 w[P], b[P], pw[P], pb[P], gate[P];
+    lane.param(a.weight, a.param_code, 1.0f, w);
+    lane.param(a.post_weight, a.param_code, 1.0f, pw);
+    if (FULL) {
+        lane.param(a.bias, a.param_code, 0.0f, b);
+        lane.param(a.post_bias, a.param_code, 0.0f, pb);
+    }
+    lane.fill(a.scale, gate);
+    while (walk.row < walk.hi) {
+        if (walk.next()) {
+            lane.param(static_cast<const char*>(a.gate) + walk.group * a.d * param_bytes(a.gate_code), a.gate_code,
+                       1.0f, gate);
+            #pragma unroll
+            for (int e = 0; e < P; ++e) gate[e] = mul2(gate[e], both(a.scale));
+        }
+        feed_wait(walk.slots - R);
+        float2 u[R][P], r[R][P];
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (i < walk.count) {
+                const uint32_t at = walk.slot_of(i) * per_slot;
+                from_update.get(lane, walk.row + i, at, u[i]);
+                from_residual.get(lane, walk.row + i, at, r[i]);
+            } else {
+                lane.fill(0.0f, u[i]);
+                lane.fill(0.0f, r[i]);
+            }
+        }
+        walk.ahead(walk.count, fetch);
+        float mean[R] = {}, rstd[R], post_mean[R] = {}, post_rstd[R];
+        #pragma unroll
+        for (int i = 0; i < R; ++i) rstd[i] = post_rstd[i] = 1.0f;
+        if (a.post_weight) {
+            if (FULL && a.layer) row_stats<true>(lane, u, inv_d, a.eps, reduce, post_mean, post_rstd);
+            else row_stats<false>(lane, u, inv_d, a.eps, reduce, post_mean, post_rstd);
+            #pragma unroll
+            for (int i = 0; i < R; ++i) {
+                #pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    u[i][e] = mul2(u[i][e], both(post_rstd[i]));
+                    u[i][e] = FULL ? fma2(u[i][e], pw[e], pb[e]) : mul2(u[i][e], pw[e]);
+                }
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            #pragma unroll
+            for (int e = 0; e < P; ++e) {
+                r[i][e] = fma2(gate[e], u[i][e], r[i][e]);
+                if (sizeof(TS) != 4) {       // the norm that follows is that of the stream as it is stored
+                    r[i][e].x = gb_up(gb_down<TS>(r[i][e].x));
+                    r[i][e].y = gb_up(gb_down<TS>(r[i][e].y));
+                }
+            }
+            if (FULL) lane.mask(r[i]);
+            if (i < walk.count) lane.store(static_cast<TS*>(a.stream) + (walk.row + i) * a.d, r[i]);
+        }
+        if (a.next) {
+            if (FULL && a.layer) row_stats<true>(lane, r, inv_d, a.eps, reduce, mean, rstd);
+            else row_stats<false>(lane, r, inv_d, a.eps, reduce, mean, rstd);
+            #pragma unroll
+            for (int i = 0; i < R; ++i) {
+                #pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    r[i][e] = mul2(r[i][e], both(rstd[i]));
+                    r[i][e] = FULL ? fma2(r[i][e], w[e], b[e]) : mul2(r[i][e], w[e]);
+                }
+                if (i < walk.count) lane.store(static_cast<TY*>(a.normed) + (walk.row + i) * a.d, r[i]);
+            }
+        }
+        if (a.stats && threadIdx.x == 0) {
+            #pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < walk.count) a.stats[walk.row + i] = make_float4(post_mean[i], post_rstd[i], mean[i], rstd[i]);
+        }
+        walk.done();
+    }
+}
+
+// The sums over R rows that norm' needs: of g x^, and in a layer norm of g.
+template <bool FULL, int P, int R>
+__device__ void backward_sums(const float2 (&g)[R][P], const float2 (&hat)[R][P], int layer, float inv_d,
+                              Reducer& reduce, float (&m1)[R], float (&m0)[R]) {
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+        float2 s = mul2(g[i][0], hat[i][0]);
+        #pragma unroll
+        for (int e = 1; e < P; ++e) s = fma2(g[i][e], hat[i][e], s);
+        m1[i] = s.x + s.y;
+        m0[i] = 0.0f;
+    }
+    if (FULL && layer) {
+        float all[2 * R];
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float2 s = g[i][0];
+            #pragma unroll
+            for (int e = 1; e < P; ++e) s = add2(s, g[i][e]);
+            all[2 * i] = m1[i];
+            all[2 * i + 1] = s.x + s.y;
+        }
+        reduce.sum(all);
+        #pragma unroll
+        for (int i = 0; i < R; ++i) { m1[i] = all[2 * i]; m0[i] = all[2 * i + 1] * inv_d; }
+    } else reduce.sum(m1);
+    #pragma unroll
+    for (int i = 0; i < R; ++i) m1[i] *= inv_d;
 }
 
 // One block is one worker.  part[worker] holds, one behind the other, the sums of d_weight,
 // d_bias, d_post_weight, d_post_bias that exist.  Worker c and gate group g meet in slot c + g of
 // gate_part: along the rows one of the two grows by one at a time, so no two pairs share a slot.
 // NEXT: the following norm's gradient takes part; OWN: the update has a norm or a gate of its own.
-template <typename TS, typename TU, typename TY, int VEC, int NV, bool NEXT, bool OWN>
+template <typename TS, typename TU, typename TY, int VEC, int NV, int R, bool FULL, bool NEXT, bool OWN>
 __global__ void __launch_bounds__(MAX_THREADS) join_bwd_kernel(const JoinArgs a) {
-    __shared__ float2 buffer[2 * MAX_WARPS];
-    Reducer reduce{buffer};
-    const Lane<VEC, NV> lane(a.d);
+    __shared__ __align__(16) float buffer[2 * MAX_WARPS * 4];
+    using L = Lane<VEC, NV>;
+    constexpr int P = L::P;
+    const L lane(a.d);
     using FS = Feed<TS, VEC, NV>;
     using FU = Feed<TU, VEC, NV>;
     using FY = Feed<TY, VEC, NV>;
@@ -373,112 +487,174 @@ __global__ void __launch_bounds__(MAX_THREADS) join_bwd_kernel(const JoinArgs a)
     FU from_update;
     FY from_normed;
     constexpr int BYTES = FS::BYTES + (NEXT ? FS::BYTES + FY::BYTES : 0) + (OWN ? FU::BYTES : 0);
-    const uint32_t per_stage = BYTES * blockDim.x;
+    const uint32_t per_slot = BYTES * blockDim.x;
     uint32_t region = (uint32_t)__cvta_generic_to_shared(join_shared);
-    from_grad.place(a.d_stream, a.d, region, per_stage);
+    from_grad.place(a.d_stream, a.d, region);
     region += FS::BYTES * blockDim.x;
     if (NEXT) {
-        from_stream.place(a.stream, a.d, region, per_stage);
+        from_stream.place(a.stream, a.d, region);
         region += FS::BYTES * blockDim.x;
-        from_normed.place(a.d_normed, a.d, region, per_stage);
+        from_normed.place(a.d_normed, a.d, region);
         region += FY::BYTES * blockDim.x;
     }
-    if (OWN) from_update.place(a.update, a.update_stride, region, per_stage);
-    const long long worker = blockIdx.x;
-    const long long lo = first_row(worker, a.rows, gridDim.x), hi = first_row(worker + 1, a.rows, gridDim.x);
-    auto fetch = [&](long long row, int stage) {
-        if (row < hi) {
-            if (a.d_stream) from_grad.fetch(lane, row, stage);
-            if (NEXT) {
-                from_stream.fetch(lane, row, stage);
-                from_normed.fetch(lane, row, stage);
-            }
-            if (OWN) from_update.fetch(lane, row, stage);
+    if (OWN) from_update.place(a.update, a.update_stride, region);
+    Walk<R> walk(a);
+    auto fetch = [&](long long row, int slot) {
+        const uint32_t at = slot * per_slot;
+        if (a.d_stream) from_grad.fetch(lane, row, at);
+        if (NEXT) {
+            from_stream.fetch(lane, row, at);
+            from_normed.fetch(lane, row, at);
         }
-        feed_commit();
+        if (OWN) from_update.fetch(lane, row, at);
     };
-    for (int i = 0; i < a.stages - 1; ++i) fetch(lo + i, i);
-    float w[NV][VEC], pw[NV][VEC], pb[NV][VEC];
-    float dw[NV][VEC], db[NV][VEC], dpw[NV][VEC], dpb[NV][VEC], dg[NV][VEC];
+    walk.ahead(walk.slots, fetch);
+    Reducer reduce(buffer);
+    const float inv_d = 1.0f / (float)a.d;
+    float2 w[P], pw[P], pb[P], gate[P];
+    float2 dw[P], db[P], dpw[P], dpb[P], dg[P];
     lane.param(a.weight, a.param_code, 1.0f, w);
     lane.param(a.post_weight, a.param_code, 1.0f, pw);
-    lane.param(a.post_bias, a.param_code, 0.0f, pb);
-    Gate<VEC, NV> gate;
+    lane.fill(a.scale, gate);
     lane.fill(0.0f, dw);
-    lane.fill(0.0f, db);
     lane.fill(0.0f, dpw);
-    lane.fill(0.0f, dpb);
     lane.fill(0.0f, dg);
-    int stage = 0;
-    for (long long row = lo; row < hi; ++row) {
-        const int ahead = stage == 0 ? a.stages - 1 : stage - 1;
-        fetch(row + a.stages - 1, ahead);
-        const float4 st = a.stats[row];
-        if (OWN && a.gate) {
-            const long long before = gate.group;
-            if (gate.move(a, lane, row, 1) && before >= 0) {
-                lane.sums(a.gate_part + (worker + before) * a.d, dg);
-                lane.fill(0.0f, dg);
-            }
-        }
-        feed_wait(a.stages - 1);
-        float dr[NV][VEC];
-        if (a.d_stream) from_grad.get(lane, row, stage, dr);
-        else lane.fill(0.0f, dr);
-        if (NEXT) {
-            float g[NV][VEC], hat[NV][VEC];
-            from_normed.get(lane, row, stage, g);
-            from_stream.get(lane, row, stage, hat);
+    if (FULL) {
+        lane.param(a.post_bias, a.param_code, 0.0f, pb);
+        lane.fill(0.0f, db);
+        lane.fill(0.0f, dpb);
+    }
+    // d_gate is gathered without the scale, which is put on where it is stored
+    auto flush = [&](long long group) {
+        #pragma unroll
+        for (int e = 0; e < P; ++e) dg[e] = mul2(dg[e], both(a.scale));
+        lane.store(a.gate_part + (blockIdx.x + group) * a.d, dg);
+        lane.fill(0.0f, dg);
+    };
+    while (walk.row < walk.hi) {
+        const long long before = walk.group;
+        const bool fresh = walk.next();
+        if (OWN && fresh) {
+            if (before >= 0) flush(before);
+            lane.param(static_cast<const char*>(a.gate) + walk.group * a.d * param_bytes(a.gate_code), a.gate_code,
+                       1.0f, gate);
             #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    hat[k][j] = (hat[k][j] - st.z) * st.w;
-                    dw[k][j] += g[k][j] * hat[k][j];
-                    db[k][j] += g[k][j];
-                    g[k][j] *= w[k][j];
+            for (int e = 0; e < P; ++e) gate[e] = mul2(gate[e], both(a.scale));
+        }
+        float4 st[R];
+        #pragma unroll
+        for (int i = 0; i < R; ++i) st[i] = i < walk.count ? a.stats[walk.row + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        feed_wait(walk.slots - R);
+        float2 dr[R][P], u[R][P];
+        #pragma unroll
+        for (int i = 0; i < R; ++i) {
+            lane.fill(0.0f, dr[i]);
+            if (i < walk.count && a.d_stream) from_grad.get(lane, walk.row + i, walk.slot_of(i) * per_slot, dr[i]);
+        }
+        if (NEXT) {
+            float2 g[R][P], hat[R][P];
+            float m1[R], m0[R];
+            #pragma unroll
+            for (int i = 0; i < R; ++i) {
+                lane.fill(0.0f, g[i]);
+                lane.fill(0.0f, hat[i]);
+                if (i < walk.count) {
+                    const uint32_t at = walk.slot_of(i) * per_slot;
+                    from_normed.get(lane, walk.row + i, at, g[i]);
+                    from_stream.get(lane, walk.row + i, at, hat[i]);
                 }
             }
-            norm_backward(lane, g, hat, st.w, a.d, a.layer, reduce);
+            if (!OWN) walk.ahead(walk.count, fetch);
             #pragma unroll
-            for (int k = 0; k < NV; ++k) {
+            for (int i = 0; i < R; ++i) {
+                if (FULL && a.layer) {
+                    #pragma unroll
+                    for (int e = 0; e < P; ++e) hat[i][e] = add2(hat[i][e], both(-st[i].z));
+                    lane.mask(hat[i]);
+                }
                 #pragma unroll
-                for (int j = 0; j < VEC; ++j) dr[k][j] += g[k][j];
+                for (int e = 0; e < P; ++e) {
+                    hat[i][e] = mul2(hat[i][e], both(st[i].w));
+                    dw[e] = fma2(g[i][e], hat[i][e], dw[e]);
+                    if (FULL) db[e] = add2(db[e], g[i][e]);
+                    g[i][e] = mul2(g[i][e], w[e]);
+                }
             }
-        }
-        if (a.d_residual) lane.store(static_cast<TS*>(a.d_residual) + row * a.d, dr);
-        #pragma unroll
-        for (int k = 0; k < NV; ++k) {
+            backward_sums<FULL>(g, hat, a.layer, inv_d, reduce, m1, m0);
             #pragma unroll
-            for (int j = 0; j < VEC; ++j) dr[k][j] *= a.scale;
+            for (int i = 0; i < R; ++i) {
+                const float2 rs = both(st[i].w), back = both(-m1[i] * st[i].w);
+                #pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    if (FULL) g[i][e] = add2(g[i][e], both(-m0[i]));
+                    dr[i][e] = fma2(g[i][e], rs, fma2(hat[i][e], back, dr[i][e]));
+                }
+                if (FULL) lane.mask(dr[i]);
+            }
         }
         if (OWN) {
-            float u[NV][VEC];
-            from_update.get(lane, row, stage, u);
             #pragma unroll
-            for (int k = 0; k < NV; ++k) {
+            for (int i = 0; i < R; ++i) {
+                lane.fill(0.0f, u[i]);
+                if (i < walk.count) from_update.get(lane, walk.row + i, walk.slot_of(i) * per_slot, u[i]);
+            }
+        }
+        if (OWN || !NEXT) walk.ahead(walk.count, fetch);
+        if (a.d_residual) {
+            #pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < walk.count) lane.store(static_cast<TS*>(a.d_residual) + (walk.row + i) * a.d, dr[i]);
+        }
+        if (OWN) {
+            #pragma unroll
+            for (int i = 0; i < R; ++i) {
+                if (FULL && a.layer && a.post_weight) {
+                    #pragma unroll
+                    for (int e = 0; e < P; ++e) u[i][e] = add2(u[i][e], both(-st[i].x));
+                    lane.mask(u[i]);
+                }
                 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    u[k][j] = (u[k][j] - st.x) * st.y;            // the update itself without a post norm
-                    dg[k][j] += dr[k][j] * (u[k][j] * pw[k][j] + pb[k][j]);
-                    dr[k][j] *= gate.v[k][j];
-                    dpw[k][j] += dr[k][j] * u[k][j];
-                    dpb[k][j] += dr[k][j];
-                    dr[k][j] *= pw[k][j];
+                for (int e = 0; e < P; ++e) {
+                    u[i][e] = mul2(u[i][e], both(st[i].y));            // the update itself without a post norm
+                    const float2 v = FULL ? fma2(u[i][e], pw[e], pb[e]) : mul2(u[i][e], pw[e]);
+                    dg[e] = fma2(dr[i][e], v, dg[e]);
+                    dr[i][e] = mul2(dr[i][e], gate[e]);
+                    dpw[e] = fma2(dr[i][e], u[i][e], dpw[e]);
+                    if (FULL) dpb[e] = add2(dpb[e], dr[i][e]);
+                    dr[i][e] = mul2(dr[i][e], pw[e]);
                 }
             }
-            if (a.post_weight) norm_backward(lane, dr, u, st.y, a.d, a.layer, reduce);
+            if (a.post_weight) {
+                float m1[R], m0[R];
+                backward_sums<FULL>(dr, u, a.layer, inv_d, reduce, m1, m0);
+                #pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    #pragma unroll
+                    for (int e = 0; e < P; ++e) {
+                        if (FULL) dr[i][e] = add2(dr[i][e], both(-m0[i]));
+                        dr[i][e] = mul2(both(st[i].y), fma2(u[i][e], both(-m1[i]), dr[i][e]));
+                    }
+                }
+            }
+        } else {
+            #pragma unroll
+            for (int i = 0; i < R; ++i) {
+                #pragma unroll
+                for (int e = 0; e < P; ++e) dr[i][e] = mul2(dr[i][e], gate[e]);
+            }
         }
-        lane.store(static_cast<TU*>(a.d_update) + row * a.d, dr);
-        stage = stage + 1 == a.stages ? 0 : stage + 1;
+        #pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i < walk.count) lane.store(static_cast<TU*>(a.d_update) + (walk.row + i) * a.d, dr[i]);
+        walk.done();
     }
-    if (OWN && a.gate && gate.group >= 0) lane.sums(a.gate_part + (worker + gate.group) * a.d, dg);
+    if (OWN && a.gate && walk.group >= 0) flush(walk.group);
     const int sums = (NEXT ? (a.bias ? 2 : 1) : 0) + (a.post_weight ? (a.post_bias ? 2 : 1) : 0);
-    float* mine = a.part + worker * sums * a.d;
-    if (NEXT) { lane.sums(mine, dw); mine += a.d; }
-    if (NEXT && a.bias) { lane.sums(mine, db); mine += a.d; }
-    if (OWN && a.post_weight) { lane.sums(mine, dpw); mine += a.d; }
-    if (OWN && a.post_weight && a.post_bias) lane.sums(mine, dpb);
+    float* mine = a.part + (size_t)blockIdx.x * sums * a.d;
+    if (NEXT) { lane.store(mine, dw); mine += a.d; }
+    if (FULL && NEXT && a.bias) { lane.store(mine, db); mine += a.d; }
+    if (OWN && a.post_weight) { lane.store(mine, dpw); mine += a.d; }
+    if (FULL && OWN && a.post_weight && a.post_bias) lane.store(mine, dpb);
 }
 
 struct SumArgs {
@@ -490,8 +666,9 @@ struct SumArgs {
     int d, sums, param_code, gate_code;
 };
 
-// Column sums of the partial results: 32 columns a block, SLICES threads share a column.
-constexpr int SLICES = 16;
+// Column sums of the partial results: 32 columns a block, SLICES threads share a column, four
+// partial results under way in each.
+constexpr int SLICES = 32;
 __global__ void __launch_bounds__(32 * SLICES) join_sum_kernel(const SumArgs a) {
     const int col = blockIdx.y * 32 + threadIdx.x;
     const long long which = blockIdx.x;
@@ -509,15 +686,26 @@ __global__ void __launch_bounds__(32 * SLICES) join_sum_kernel(const SumArgs a) 
         stride = a.d;
     }
     float acc = 0.0f;
-    if (col < a.d) for (long long c = lo + threadIdx.y; c < hi; c += SLICES) acc += base[c * stride + col];
+    if (col < a.d) {
+        long long c = lo + threadIdx.y;
+        for (; c + 3 * SLICES < hi; c += 4 * SLICES) {
+            float v[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = base[(c + i * SLICES) * stride + col];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) acc += v[i];
+        }
+        for (; c < hi; c += SLICES) acc += base[c * stride + col];
+    }
     __shared__ float slice[SLICES][33];
     slice[threadIdx.y][threadIdx.x] = acc;
     __syncthreads();
-    if (threadIdx.y == 0 && col < a.d) {
-        float total = slice[0][threadIdx.x];
-        for (int s = 1; s < SLICES; ++s) total += slice[s][threadIdx.x];
-        if (which < a.sums) gb_write(a.out[which], a.param_code, col, total);
-        else gb_write(a.gate_out, a.gate_code, (size_t)(which - a.sums) * a.d + col, total);
+    // warp y sums column y of the block
+    const float total = gb_warp_sum(slice[threadIdx.x][threadIdx.y]);
+    const int mine = blockIdx.y * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && mine < a.d) {
+        if (which < a.sums) gb_write(a.out[which], a.param_code, mine, total);
+        else gb_write(a.gate_out, a.gate_code, (size_t)(which - a.sums) * a.d + mine, total);
     }
 }
 
@@ -546,16 +734,16 @@ int workers_for(long long rows, int threads) {
     return (int)(rows < most ? rows : most);
 }
 
-// Stages that fit beside one another in an SM's 227 KB.
-int stages_for(int bytes_per_stage, int blocks) {
-    int n = bytes_per_stage ? (int)((220 << 10) / blocks / bytes_per_stage) : MAX_STAGES;
-    return n < 1 ? 1 : n > MAX_STAGES ? MAX_STAGES : n;
+// Slots that fit beside one another in an SM's 227 KB.
+int slots_for(int bytes_per_slot, int blocks, int rows_at_once) {
+    int n = bytes_per_slot ? (int)((220 << 10) / blocks / bytes_per_slot) : MAX_SLOTS;
+    return n < rows_at_once ? rows_at_once : n > MAX_SLOTS ? MAX_SLOTS : n;
 }
 
 template <typename K>
-int start(K kernel, int grid, int threads, int bytes_per_stage, int blocks, JoinArgs a, cudaStream_t s) {
-    a.stages = stages_for(bytes_per_stage, blocks);
-    const int shared = a.stages * bytes_per_stage;
+int start(K kernel, int grid, int threads, int bytes_per_slot, int blocks, int rows_at_once, JoinArgs a, cudaStream_t s) {
+    a.slots = slots_for(bytes_per_slot, blocks, rows_at_once);
+    const int shared = a.slots * bytes_per_slot;
     if (shared > (40 << 10)) {                       // more than a launch may take unasked, with the static part
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
         if (err != cudaSuccess) return (int)err;
@@ -564,28 +752,34 @@ int start(K kernel, int grid, int threads, int bytes_per_stage, int blocks, Join
     return (int)cudaGetLastError();
 }
 
-template <typename TS, typename TU, typename TY, int VEC, int NV>
-int launch_shaped(bool forward, int threads, const JoinArgs& a, cudaStream_t s) {
+template <typename TS, typename TU, typename TY, int VEC, int NV, int R, bool FULL>
+int launch_form(bool forward, int threads, const JoinArgs& a, cudaStream_t s) {
     constexpr int S = Feed<TS, VEC, NV>::BYTES, U = Feed<TU, VEC, NV>::BYTES, Y = Feed<TY, VEC, NV>::BYTES;
     const int blocks = blocks_per_sm(threads);
     const int grid = workers_for(a.rows, threads);
-    if (forward) return start(join_fwd_kernel<TS, TU, TY, VEC, NV>, grid, threads, (S + U) * threads, blocks, a, s);
+    if (forward) return start(join_fwd_kernel<TS, TU, TY, VEC, NV, R, FULL>, grid, threads, (S + U) * threads, blocks, R, a, s);
     const bool next = a.d_normed, own = a.post_weight || a.gate;
-    if (next && own) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, true, true>, grid, threads, (2 * S + Y + U) * threads, blocks, a, s);
-    if (next) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, true, false>, grid, threads, (2 * S + Y) * threads, blocks, a, s);
-    return start(join_bwd_kernel<TS, TU, TY, VEC, NV, false, true>, grid, threads, (S + U) * threads, blocks, a, s);
+    if (next && own) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, R, FULL, true, true>, grid, threads, (2 * S + Y + U) * threads, blocks, R, a, s);
+    if (next) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, R, FULL, true, false>, grid, threads, (2 * S + Y) * threads, blocks, R, a, s);
+    return start(join_bwd_kernel<TS, TU, TY, VEC, NV, R, FULL, false, true>, grid, threads, (S + U) * threads, blocks, R, a, s);
+}
+
+template <typename TS, typename TU, typename TY, int VEC, int NV, int R>
+int launch_shaped(bool forward, int threads, const JoinArgs& a, cudaStream_t s) {
+    if (a.layer || a.bias || a.post_bias) return launch_form<TS, TU, TY, VEC, NV, R, true>(forward, threads, a, s);
+    return launch_form<TS, TU, TY, VEC, NV, R, false>(forward, threads, a, s);
 }
 
 template <typename TS, typename TU, typename TY>
 int launch(bool forward, int vec, const JoinArgs& a, cudaStream_t s) {
     const Shape shape = shape_of(a.d, vec);
     if (vec == 8) {
-        if (shape.rounds == 1) return launch_shaped<TS, TU, TY, 8, 1>(forward, shape.threads, a, s);
-        return launch_shaped<TS, TU, TY, 8, 2>(forward, shape.threads, a, s);
+        if (shape.rounds == 1) return launch_shaped<TS, TU, TY, 8, 1, 2>(forward, shape.threads, a, s);
+        return launch_shaped<TS, TU, TY, 8, 2, 1>(forward, shape.threads, a, s);
     }
-    if (shape.rounds <= 1) return launch_shaped<TS, TU, TY, 1, 1>(forward, shape.threads, a, s);
-    if (shape.rounds <= 4) return launch_shaped<TS, TU, TY, 1, 4>(forward, shape.threads, a, s);
-    return launch_shaped<TS, TU, TY, 1, 16>(forward, shape.threads, a, s);
+    if (shape.rounds <= 1) return launch_shaped<TS, TU, TY, 1, 1, 2>(forward, shape.threads, a, s);
+    if (shape.rounds <= 4) return launch_shaped<TS, TU, TY, 1, 4, 2>(forward, shape.threads, a, s);
+    return launch_shaped<TS, TU, TY, 1, 16, 1>(forward, shape.threads, a, s);
 }
 
 int dispatch(bool forward, int s, int u, int y, int vec, const JoinArgs& a, cudaStream_t stream) {
