@@ -36,11 +36,16 @@ struct JoinArgs {
     float* gate_part;                  // [workers + groups - 1][d]
     long long rows, group_rows;        // rows of one gate group
     int d, layer, param_code, gate_code, next, slots;
+    int owners;                        // teams that have rows, at least one each
     float scale, eps;
 };
 
 constexpr int MAX_THREADS = 512;
-constexpr int MAX_WARPS = MAX_THREADS / 32;
+constexpr int REDUCER_FLOATS = 2 * 2 * (MAX_THREADS / 32) * 4;   // three warps a team take the room of four
+
+// A block is blockDim.y teams of blockDim.x threads; a team owns a row.  An SM holds one block, so
+// that a backward pass leaves one row of partial sums for each SM.
+__device__ __forceinline__ int team_of_grid() { return blockIdx.x * blockDim.y + threadIdx.y; }
 
 // Two values in one instruction (sm_100a's packed fp32); each rounds as the single one does.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -64,15 +69,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Sums of Q values over the block's threads, one barrier a reduction: the buffers alternate.
-// Within a warp the values are exchanged for one another before they are added, so that Q = 1, 2,
-// 4 cost five, five and six shuffles.
+// Sums of Q values over a team's threads, one barrier a reduction: the buffers alternate.  Within
+// a warp the values are exchanged for one another before they are added, so that Q = 1, 2, 4 cost
+// five, five and six shuffles.
 struct Reducer {
-    float* buffer;                     // [2][MAX_WARPS][4]
-    int warps, parity;
-    __device__ explicit Reducer(float* b) : buffer(b), warps((int)blockDim.x >> 5), parity(0) {
-        for (int i = threadIdx.x; i < 2 * MAX_WARPS * 4; i += blockDim.x) b[i] = 0.0f;
-        __syncthreads();
+    float* buffer;                     // [2][warps, to a multiple of four][4]
+    int warps, half, parity;
+    __device__ explicit Reducer(float* b) : warps((int)blockDim.x >> 5), half((warps + 3) / 4 * 16), parity(0) {
+        buffer = b + threadIdx.y * 2 * half;
+        if (warps == 1) return;
+        for (int i = threadIdx.x; i < 2 * half; i += blockDim.x) buffer[i] = 0.0f;
+        team_barrier();
+    }
+    __device__ static void team_barrier() {
+        asm volatile("bar.sync %0, %1;" :: "r"((int)threadIdx.y + 1), "r"((int)blockDim.x) : "memory");
     }
     template <int Q>
     __device__ void sum(float (&v)[Q]) {
@@ -96,10 +106,15 @@ struct Reducer {
         #pragma unroll
         for (int step = Q == 4 ? 4 : Q == 2 ? 8 : 16; step > 0; step >>= 1)
             mine += __shfl_xor_sync(0xffffffffu, mine, step);
-        float* b = buffer + parity * MAX_WARPS * 4;
+        if (warps == 1) {
+            #pragma unroll
+            for (int q = 0; q < Q; ++q) v[q] = Q == 1 ? mine : __shfl_sync(0xffffffffu, mine, q * (32 / Q));
+            return;
+        }
+        float* b = buffer + parity * half;
         parity ^= 1;
         if (lane % (32 / Q) == 0) b[(threadIdx.x >> 5) * Q + lane / (32 / Q)] = mine;
-        if (warps == 1) __syncwarp(); else __syncthreads();
+        team_barrier();
         // all partial results, four warps at a time (there are zeros behind the last)
         const float4* b4 = reinterpret_cast<const float4*>(b);
         #pragma unroll
@@ -115,6 +130,17 @@ struct Reducer {
         }
     }
 };
+
+// Two values rounded to T, as floats.
+template <typename T> __device__ __forceinline__ float2 rounded(float2 v) { return v; }
+template <> __device__ __forceinline__ float2 rounded<__nv_bfloat16>(float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    const uint32_t w = reinterpret_cast<const uint32_t&>(h);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 rounded<__half>(float2 v) {
+    return __half22float2(__floats2half2_rn(v.x, v.y));
+}
 
 // A thread's place in a row: vector k of NV starts at column (k * blockDim.x + threadIdx.x) * VEC.
 // Its values are held in pairs: value e of the thread is that of vector e / VEC.
@@ -159,16 +185,23 @@ struct Lane {
     __device__ void param(const void* p, int code, float otherwise, float2 (&v)[P]) const {
         fill(otherwise, v);
         if (!p) return;
+        if (code == GB_F32) read(static_cast<const float*>(p), v);
+        else if (code == GB_BF16) read(static_cast<const __nv_bfloat16*>(p), v);
+        else read(static_cast<const __half*>(p), v);
+    }
+    template <typename T>
+    __device__ void read(const T* p, float2 (&v)[P]) const {
         #pragma unroll
-        for (int e = 0; e < E; ++e) if (ok[e / VEC]) at(v, e) = gb_read(p, code, col[e / VEC] + e % VEC);
+        for (int e = 0; e < E; ++e) if (ok[e / VEC]) at(v, e) = gb_up(p[col[e / VEC] + e % VEC]);
     }
 };
 
 // Rows of one tensor on their way to this thread's registers.  Each thread copies the values that
 // it will use itself into its own places in shared memory (cp.async), as many rows ahead as there
 // are slots, so the loads of several rows are in flight while a row is reduced, no register holds
-// them and no barrier guards them.  Single values of two bytes cannot be copied so: they are read
-// when used.
+// them and no barrier guards them.  A copy of no bytes fills its place with zeros and reads
+// nothing: so it is for columns and rows that do not exist.  Single values of two bytes cannot be
+// copied so: they are read when used.
 template <typename T, int VEC, int NV>
 struct Feed {
     static constexpr bool STAGED = VEC == 8 || sizeof(T) == 4;
@@ -176,68 +209,87 @@ struct Feed {
     static constexpr int PIECES = VEC == 8 ? (int)sizeof(T) / 2 : 1;    // copies a vector
     static constexpr int BYTES = STAGED ? NV * PIECES * PIECE : 0;      // a thread and slot
     using L = Lane<VEC, NV>;
-    const T* base;
-    long long stride;
-    uint32_t at;                       // shared address of this thread's first piece of slot 0
-    __device__ void place(const void* p, long long row_stride, uint32_t region) {
-        base = static_cast<const T*>(p);
-        stride = row_stride;
-        at = region + threadIdx.x * PIECE;
+    const char* ahead;                 // this thread's first value of the next row to fetch
+    const char* here;                  // of the row at hand, where rows are not staged
+    long long step;                    // bytes from row to row
+    uint32_t place;                    // of this thread's first piece in a slot
+    __device__ void open(const void* p, long long row_stride, long long row, uint32_t region) {
+        step = row_stride * (long long)sizeof(T);
+        ahead = here = static_cast<const char*>(p) + row * step + threadIdx.x * (VEC * (int)sizeof(T));
+        place = region + threadIdx.x * PIECE;
     }
-    __device__ void fetch(const L& lane, long long row, uint32_t slot_offset) const {
+    __device__ void fetch(const L& lane, uint32_t slot, bool exists) {
         if constexpr (STAGED) {
-            const T* from = base + row * stride;
             #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (!lane.ok[k]) continue;
+                const int bytes = exists && lane.ok[k] ? PIECE : 0;
                 #pragma unroll
                 for (int h = 0; h < PIECES; ++h) {
-                    const uint32_t to = at + slot_offset + (k * PIECES + h) * blockDim.x * PIECE;
-                    const T* src = from + lane.col[k] + h * (16 / (int)sizeof(T));
+                    const uint32_t to = place + slot + (k * PIECES + h) * (int)blockDim.x * PIECE;
+                    const char* from = ahead + (long long)(k * (int)blockDim.x * (VEC * (int)sizeof(T)) + h * 16);
                     if constexpr (PIECE == 16)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(src) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(bytes) : "memory");
                     else
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(to), "l"(src) : "memory");
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" :: "r"(to), "l"(from), "r"(bytes) : "memory");
                 }
             }
+            ahead += step;
         }
     }
-    __device__ void get(const L& lane, long long row, uint32_t slot_offset, float2 (&v)[L::P]) const {
+    __device__ void get(const L& lane, uint32_t slot, float2 (&v)[L::P]) {
         if (L::E & 1) v[L::P - 1].y = 0.0f;
         #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if constexpr (VEC == 8) {
-                float f[8] = {};
-                if (lane.ok[k]) {
-                    #pragma unroll
-                    for (int h = 0; h < PIECES; ++h) {
-                        const uint32_t from = at + slot_offset + (k * PIECES + h) * blockDim.x * PIECE;
-                        uint4 q;
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(from) : "memory");
-                        if constexpr (sizeof(T) == 4) {
-                            f[4 * h] = __uint_as_float(q.x); f[4 * h + 1] = __uint_as_float(q.y);
-                            f[4 * h + 2] = __uint_as_float(q.z); f[4 * h + 3] = __uint_as_float(q.w);
-                        } else {
-                            Raw8<T> raw;
-                            raw.q = q;
-                            raw.get(f);
-                        }
+                float f[8];
+                #pragma unroll
+                for (int h = 0; h < PIECES; ++h) {
+                    uint4 q;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                                 : "r"(place + slot + (k * PIECES + h) * (int)blockDim.x * PIECE) : "memory");
+                    if constexpr (sizeof(T) == 4) {
+                        f[4 * h] = __uint_as_float(q.x); f[4 * h + 1] = __uint_as_float(q.y);
+                        f[4 * h + 2] = __uint_as_float(q.z); f[4 * h + 3] = __uint_as_float(q.w);
+                    } else {
+                        Raw8<T> raw;
+                        raw.q = q;
+                        raw.get(f);
                     }
                 }
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) L::at(v, k * 8 + j) = f[j];
-            } else {
-                float f = 0.0f;
-                if (lane.ok[k]) {
-                    if constexpr (STAGED)
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f)
-                                     : "r"(at + slot_offset + k * blockDim.x * PIECE) : "memory");
-                    else f = gb_up(base[row * stride + lane.col[k]]);
-                }
+            } else if constexpr (STAGED) {
+                float f;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(place + slot + k * (int)blockDim.x * PIECE) : "memory");
                 L::at(v, k) = f;
+            } else {
+                const T* row = reinterpret_cast<const T*>(here);
+                L::at(v, k) = lane.ok[k] ? gb_up(row[k * (int)blockDim.x]) : 0.0f;
             }
         }
+        if constexpr (!STAGED) here += step;
+    }
+};
+
+// Rows of a result, one behind the other.
+template <typename T, int VEC, int NV>
+struct Sink {
+    using L = Lane<VEC, NV>;
+    T* at;
+    __device__ void open(void* p, long long row, int d) { at = static_cast<T*>(p) + row * d + threadIdx.x * VEC; }
+    __device__ void put(const L& lane, const float2 (&v)[L::P], int d) {
+        #pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (!lane.ok[k]) continue;
+            if constexpr (VEC == 8) {
+                float f[8];
+                #pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = L::at(v, k * 8 + j);
+                gb_store8(at + k * (int)blockDim.x * 8, f);
+            } else at[k * (int)blockDim.x] = gb_down<T>(L::at(v, k));
+        }
+        at += d;
     }
 };
 
@@ -248,15 +300,12 @@ __device__ __forceinline__ void feed_wait(int behind) {
         case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
         case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
         case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
     }
 }
-constexpr int MAX_SLOTS = 8;
+constexpr int MAX_SLOTS = 4;
 
-// Worker c owns the rows [first_row(c), first_row(c + 1)); owner_of is its inverse.
+// Worker (team) c owns the rows [first_row(c), first_row(c + 1)); owner_of is its inverse.
 __host__ __device__ __forceinline__ long long first_row(long long c, long long rows, long long workers) {
     return c * rows / workers;
 }
@@ -264,397 +313,405 @@ __host__ __device__ __forceinline__ long long owner_of(long long row, long long 
     return ((row + 1) * workers - 1) / rows;
 }
 
-// A worker's walk over its rows: up to R at a time, all of one gate group, with the rows behind
-// them under way.  One group of copies a row, in the rows' order, so a wait for all but the last
-// slots - R groups is a wait for the rows at hand.
-template <int R>
-struct Walk {
-    long long row, hi, fetched, group, group_end, group_rows;
-    int slots, slot, count, fetch_slot;
-    bool gated;
-    __device__ Walk(const JoinArgs& a)
-        : row(first_row(blockIdx.x, a.rows, gridDim.x)), hi(first_row(blockIdx.x + 1LL, a.rows, gridDim.x)),
-          fetched(row), group(-1), group_end(hi), group_rows(a.group_rows), slots(a.slots), slot(0), count(0),
-          fetch_slot(0), gated(a.gate != nullptr) {}
-    template <typename F>
-    __device__ void ahead(int n, F fetch) {         // the next n rows' copies; empty groups behind the last row
-        for (int i = 0; i < n; ++i) {
-            if (fetched < hi) fetch(fetched, fetch_slot);
-            feed_commit();
-            ++fetched;
-            fetch_slot = fetch_slot + 1 == slots ? 0 : fetch_slot + 1;
-        }
-    }
-    // the rows at hand are row .. row + count - 1; true where they begin another group
-    __device__ bool next() {
-        bool fresh = false;
-        if (gated && (group < 0 || row >= group_end)) {
-            group = row / group_rows;
-            group_end = (group + 1) * group_rows;
-            fresh = true;
-        }
-        const long long end = gated && group_end < hi ? group_end : hi;
-        count = end - row < R ? (int)(end - row) : R;
-        return fresh;
-    }
-    __device__ int slot_of(int i) const { const int s = slot + i; return s >= slots ? s - slots : s; }
-    __device__ void done() { row += count; slot = slot_of(count); }
-};
-
 __device__ __forceinline__ size_t param_bytes(int code) { return code == GB_F32 ? 4 : 2; }
 
-// Mean (0 for rms) and 1 / deviation of R rows.  The variance is that of the centred values, which
-// are at hand: a second reduction instead of a difference of large numbers.
-template <bool LAYER, int VEC, int NV, int R>
-__device__ void row_stats(const Lane<VEC, NV>& lane, float2 (&v)[R][Lane<VEC, NV>::P], float inv_d, float eps,
-                          Reducer& reduce, float (&mean)[R], float (&rstd)[R]) {
+// A parameter's values in a thread's columns, as fp32: in registers, or in the thread's own places
+// in shared memory, where the sums of the backward pass need the registers (8192 x 2048 with both
+// norms and a gate: spilled registers cost more than the reads).
+template <int VEC, int NV, bool SHARED>
+struct Held {
+    using L = Lane<VEC, NV>;
+    static constexpr int PIECE = VEC == 8 ? 16 : 4;
+    static constexpr int BYTES = SHARED ? L::E * 4 : 0;       // a thread
+    float2 v[SHARED ? 1 : L::P];
+    uint32_t place;
+    __device__ void set(const float2 (&x)[L::P], uint32_t region) {
+        place = region + threadIdx.x * PIECE;
+        if constexpr (!SHARED) {
+            #pragma unroll
+            for (int e = 0; e < L::P; ++e) v[e] = x[e];
+        } else if constexpr (VEC == 8) {
+            #pragma unroll
+            for (int i = 0; i < L::E / 4; ++i)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};"
+                             :: "r"(place + i * (int)blockDim.x * 16), "f"(x[2 * i].x), "f"(x[2 * i].y),
+                                "f"(x[2 * i + 1].x), "f"(x[2 * i + 1].y) : "memory");
+        } else {
+            #pragma unroll
+            for (int e = 0; e < L::E; ++e)
+                asm volatile("st.shared.f32 [%0], %1;" :: "r"(place + e * (int)blockDim.x * 4), "f"(L::at(x, e)) : "memory");
+        }
+    }
+    __device__ void get(float2 (&x)[L::P]) const {
+        if constexpr (!SHARED) {
+            #pragma unroll
+            for (int e = 0; e < L::P; ++e) x[e] = v[e];
+        } else if constexpr (VEC == 8) {
+            #pragma unroll
+            for (int i = 0; i < L::E / 4; ++i)
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x[2 * i].x), "=f"(x[2 * i].y), "=f"(x[2 * i + 1].x), "=f"(x[2 * i + 1].y)
+                             : "r"(place + i * (int)blockDim.x * 16) : "memory");
+        } else {
+            if (L::E & 1) x[L::P - 1].y = 0.0f;
+            #pragma unroll
+            for (int e = 0; e < L::E; ++e)
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(L::at(x, e)) : "r"(place + e * (int)blockDim.x * 4) : "memory");
+        }
+    }
+};
+
+// The scale times the gate of the row at hand, read where a row begins another group.
+template <int VEC, int NV, bool SHARED>
+struct Gate {
+    using L = Lane<VEC, NV>;
+    Held<VEC, NV, SHARED> held;
+    long long group = -1, end;
+    uint32_t region;
+    __device__ Gate(const JoinArgs& a, long long lo, uint32_t region_) : end(a.gate ? lo : a.rows), region(region_) {
+        float2 v[L::P];
+        L::fill(a.scale, v);
+        held.set(v, region);
+    }
+    __device__ void move(const JoinArgs& a, const L& lane, long long row) {
+        group = row / a.group_rows;
+        end = (group + 1) * a.group_rows;
+        float2 v[L::P];
+        lane.param(static_cast<const char*>(a.gate) + group * a.d * param_bytes(a.gate_code), a.gate_code, 1.0f, v);
+        #pragma unroll
+        for (int e = 0; e < L::P; ++e) v[e] = mul2(v[e], both(a.scale));
+        held.set(v, region);
+    }
+};
+
+// Mean (0 for rms) and 1 / deviation of a row, which is centred in place.  The variance is that of
+// the centred values: a second reduction instead of a difference of large numbers.
+template <bool FULL, int VEC, int NV>
+__device__ float2 row_stats(const Lane<VEC, NV>& lane, float2 (&v)[Lane<VEC, NV>::P], int layer, float inv_d,
+                            float eps, Reducer& reduce) {
     constexpr int P = Lane<VEC, NV>::P;
-    if constexpr (LAYER) {
+    float mean = 0.0f;
+    if (FULL && layer) {
+        float2 s = v[0];
         #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            float2 s = v[i][0];
-            #pragma unroll
-            for (int e = 1; e < P; ++e) s = add2(s, v[i][e]);
-            mean[i] = s.x + s.y;
-        }
-        reduce.sum(mean);
+        for (int e = 1; e < P; ++e) s = add2(s, v[e]);
+        float sum[1] = {s.x + s.y};
+        reduce.sum(sum);
+        mean = sum[0] * inv_d;
         #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            mean[i] *= inv_d;
-            #pragma unroll
-            for (int e = 0; e < P; ++e) v[i][e] = add2(v[i][e], both(-mean[i]));
-            lane.mask(v[i]);
-        }
+        for (int e = 0; e < P; ++e) v[e] = add2(v[e], both(-mean));
+        lane.mask(v);
     }
+    float2 q = mul2(v[0], v[0]);
     #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        float2 q = mul2(v[i][0], v[i][0]);
-        #pragma unroll
-        for (int e = 1; e < P; ++e) q = fma2(v[i][e], v[i][e], q);
-        rstd[i] = q.x + q.y;
-    }
-    reduce.sum(rstd);
-    #pragma unroll
-    for (int i = 0; i < R; ++i) rstd[i] = 1.0f / sqrtf(rstd[i] * inv_d + eps);
+    for (int e = 1; e < P; ++e) q = fma2(v[e], v[e], q);
+    float sum[1] = {q.x + q.y};
+    reduce.sum(sum);
+    return make_float2(mean, rsqrtf(sum[0] * inv_d + eps));          // 2 ulp
 }
 
 extern __shared__ __align__(16) char join_shared[];
 
 // FULL: layer norms, or any bias; otherwise rms norms without.
-template <typename TS, typename TU, typename TY, int VEC, int NV, int R, bool FULL>
-__global__ void __launch_bounds__(MAX_THREADS) join_fwd_kernel(const JoinArgs a) {
-    __shared__ __align__(16) float buffer[2 * MAX_WARPS * 4];
+template <typename TS, typename TU, typename TY, int VEC, int NV, bool FULL>
+__global__ void __launch_bounds__(NV == 3 ? 384 : MAX_THREADS) join_fwd_kernel(const JoinArgs a) {
+    __shared__ __align__(16) float buffer[REDUCER_FLOATS];
     using L = Lane<VEC, NV>;
     constexpr int P = L::P;
+    if (team_of_grid() >= a.owners) return;          // a team's barriers are its own
     const L lane(a.d);
+    const long long lo = first_row(team_of_grid(), a.rows, a.owners), hi = first_row(team_of_grid() + 1LL, a.rows, a.owners);
+    constexpr bool SHARED = FULL && VEC * NV > 8 && NV < 16;
+    using H = Held<VEC, NV, SHARED>;
+    const uint32_t per_slot = (Feed<TS, VEC, NV>::BYTES + Feed<TU, VEC, NV>::BYTES) * blockDim.x;
+    const uint32_t held_bytes = H::BYTES * blockDim.x;
+    // the teams' columns are the same: they share the parameters, and each has its gate and slots
+    const uint32_t held_at = (uint32_t)__cvta_generic_to_shared(join_shared);
+    const uint32_t gate_at = held_at + 4 * held_bytes + threadIdx.y * (a.slots * per_slot + held_bytes);
+    const uint32_t mine = gate_at + held_bytes;
     Feed<TS, VEC, NV> from_residual;
     Feed<TU, VEC, NV> from_update;
-    constexpr int BYTES = Feed<TS, VEC, NV>::BYTES + Feed<TU, VEC, NV>::BYTES;
-    const uint32_t shared = (uint32_t)__cvta_generic_to_shared(join_shared), per_slot = BYTES * blockDim.x;
-    from_residual.place(a.residual, a.residual_stride, shared);
-    from_update.place(a.update, a.update_stride, shared + Feed<TS, VEC, NV>::BYTES * blockDim.x);
-    Walk<R> walk(a);
-    auto fetch = [&](long long row, int slot) {
-        from_residual.fetch(lane, row, slot * per_slot);
-        from_update.fetch(lane, row, slot * per_slot);
-    };
-    walk.ahead(walk.slots, fetch);
+    from_residual.open(a.residual, a.residual_stride, lo, mine);
+    from_update.open(a.update, a.update_stride, lo, mine + Feed<TS, VEC, NV>::BYTES * blockDim.x);
+    for (int i = 0; i < a.slots; ++i) {
+        from_update.fetch(lane, i * per_slot, lo + i < hi);
+        from_residual.fetch(lane, i * per_slot, lo + i < hi);
+        feed_commit();
+    }
+    Sink<TS, VEC, NV> to_stream;
+    Sink<TY, VEC, NV> to_normed;
+    to_stream.open(a.stream, lo, a.d);
+    to_normed.open(a.normed, lo, a.d);
     Reducer reduce(buffer);
     const float inv_d = 1.0f / (float)a.d;
-    float2 w[P], b[P], pw[P], pb[P], gate[P];
-    lane.param(a.weight, a.param_code, 1.0f, w);
-    lane.param(a.post_weight, a.param_code, 1.0f, pw);
+    H weight, bias, post_weight, post_bias;
+    auto hold = [&](H& held, const void* p, float otherwise, int i) {
+        float2 v[P];
+        lane.param(p, a.param_code, otherwise, v);
+        held.set(v, held_at + i * held_bytes);
+    };
+    hold(weight, a.weight, 1.0f, 0);
+    hold(post_weight, a.post_weight, 1.0f, 1);
     if (FULL) {
-        lane.param(a.bias, a.param_code, 0.0f, b);
-        lane.param(a.post_bias, a.param_code, 0.0f, pb);
+        hold(bias, a.bias, 0.0f, 2);
+        hold(post_bias, a.post_bias, 0.0f, 3);
     }
-    lane.fill(a.scale, gate);
-    while (walk.row < walk.hi) {
-        if (walk.next()) {
-            lane.param(static_cast<const char*>(a.gate) + walk.group * a.d * param_bytes(a.gate_code), a.gate_code,
-                       1.0f, gate);
-            #pragma unroll
-            for (int e = 0; e < P; ++e) gate[e] = mul2(gate[e], both(a.scale));
-        }
-        feed_wait(walk.slots - R);
-        float2 u[R][P], r[R][P];
-        #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (i < walk.count) {
-                const uint32_t at = walk.slot_of(i) * per_slot;
-                from_update.get(lane, walk.row + i, at, u[i]);
-                from_residual.get(lane, walk.row + i, at, r[i]);
-            } else {
-                lane.fill(0.0f, u[i]);
-                lane.fill(0.0f, r[i]);
-            }
-        }
-        walk.ahead(walk.count, fetch);
-        float mean[R] = {}, rstd[R], post_mean[R] = {}, post_rstd[R];
-        #pragma unroll
-        for (int i = 0; i < R; ++i) rstd[i] = post_rstd[i] = 1.0f;
+    Gate<VEC, NV, SHARED> gate(a, lo, gate_at);
+    uint32_t slot = 0;
+    const uint32_t last_slot = (a.slots - 1) * per_slot;
+    for (long long row = lo; row < hi; ++row) {
+        if (row >= gate.end) gate.move(a, lane, row);
+        feed_wait(a.slots - 1);
+        float2 u[P], r[P];
+        from_update.get(lane, slot, u);
+        from_residual.get(lane, slot, r);
+        from_update.fetch(lane, slot, row + a.slots < hi);
+        from_residual.fetch(lane, slot, row + a.slots < hi);
+        feed_commit();
+        slot = slot == last_slot ? 0 : slot + per_slot;
+        float2 post = make_float2(0.0f, 1.0f), next = make_float2(0.0f, 1.0f);
         if (a.post_weight) {
-            if (FULL && a.layer) row_stats<true>(lane, u, inv_d, a.eps, reduce, post_mean, post_rstd);
-            else row_stats<false>(lane, u, inv_d, a.eps, reduce, post_mean, post_rstd);
-            #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    u[i][e] = mul2(u[i][e], both(post_rstd[i]));
-                    u[i][e] = FULL ? fma2(u[i][e], pw[e], pb[e]) : mul2(u[i][e], pw[e]);
-                }
-            }
-        }
-        #pragma unroll
-        for (int i = 0; i < R; ++i) {
+            post = row_stats<FULL>(lane, u, a.layer, inv_d, a.eps, reduce);
+            float2 pw[P], pb[P];
+            post_weight.get(pw);
+            if (FULL) post_bias.get(pb);
             #pragma unroll
             for (int e = 0; e < P; ++e) {
-                r[i][e] = fma2(gate[e], u[i][e], r[i][e]);
-                if (sizeof(TS) != 4) {       // the norm that follows is that of the stream as it is stored
-                    r[i][e].x = gb_up(gb_down<TS>(r[i][e].x));
-                    r[i][e].y = gb_up(gb_down<TS>(r[i][e].y));
-                }
+                u[e] = mul2(u[e], both(post.y));
+                u[e] = FULL ? fma2(u[e], pw[e], pb[e]) : mul2(u[e], pw[e]);
             }
-            if (FULL) lane.mask(r[i]);
-            if (i < walk.count) lane.store(static_cast<TS*>(a.stream) + (walk.row + i) * a.d, r[i]);
         }
+        {
+            float2 g[P];
+            gate.held.get(g);
+            #pragma unroll
+            for (int e = 0; e < P; ++e)          // the norm that follows is that of the stream as it is stored
+                r[e] = rounded<TS>(fma2(g[e], u[e], r[e]));
+        }
+        to_stream.put(lane, r, a.d);
         if (a.next) {
-            if (FULL && a.layer) row_stats<true>(lane, r, inv_d, a.eps, reduce, mean, rstd);
-            else row_stats<false>(lane, r, inv_d, a.eps, reduce, mean, rstd);
+            if (FULL) lane.mask(r);
+            next = row_stats<FULL>(lane, r, a.layer, inv_d, a.eps, reduce);
+            float2 w[P], b[P];
+            weight.get(w);
+            if (FULL) bias.get(b);
             #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    r[i][e] = mul2(r[i][e], both(rstd[i]));
-                    r[i][e] = FULL ? fma2(r[i][e], w[e], b[e]) : mul2(r[i][e], w[e]);
-                }
-                if (i < walk.count) lane.store(static_cast<TY*>(a.normed) + (walk.row + i) * a.d, r[i]);
+            for (int e = 0; e < P; ++e) {
+                r[e] = mul2(r[e], both(next.y));
+                r[e] = FULL ? fma2(r[e], w[e], b[e]) : mul2(r[e], w[e]);
             }
+            to_normed.put(lane, r, a.d);
         }
-        if (a.stats && threadIdx.x == 0) {
-            #pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (i < walk.count) a.stats[walk.row + i] = make_float4(post_mean[i], post_rstd[i], mean[i], rstd[i]);
-        }
-        walk.done();
+        if (a.stats && threadIdx.x == 0) a.stats[row] = make_float4(post.x, post.y, next.x, next.y);
     }
 }
 
-// The sums over R rows that norm' needs: of g x^, and in a layer norm of g.
-template <bool FULL, int P, int R>
-__device__ void backward_sums(const float2 (&g)[R][P], const float2 (&hat)[R][P], int layer, float inv_d,
-                              Reducer& reduce, float (&m1)[R], float (&m0)[R]) {
+// The means over a row that norm' needs: of g x^, and in a layer norm of g.
+template <bool FULL, int P>
+__device__ float2 backward_means(const float2 (&g)[P], const float2 (&hat)[P], int layer, float inv_d, Reducer& reduce) {
+    float2 s = mul2(g[0], hat[0]);
     #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        float2 s = mul2(g[i][0], hat[i][0]);
-        #pragma unroll
-        for (int e = 1; e < P; ++e) s = fma2(g[i][e], hat[i][e], s);
-        m1[i] = s.x + s.y;
-        m0[i] = 0.0f;
-    }
+    for (int e = 1; e < P; ++e) s = fma2(g[e], hat[e], s);
     if (FULL && layer) {
-        float all[2 * R];
+        float2 z = g[0];
         #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            float2 s = g[i][0];
-            #pragma unroll
-            for (int e = 1; e < P; ++e) s = add2(s, g[i][e]);
-            all[2 * i] = m1[i];
-            all[2 * i + 1] = s.x + s.y;
-        }
-        reduce.sum(all);
-        #pragma unroll
-        for (int i = 0; i < R; ++i) { m1[i] = all[2 * i]; m0[i] = all[2 * i + 1] * inv_d; }
-    } else reduce.sum(m1);
-    #pragma unroll
-    for (int i = 0; i < R; ++i) m1[i] *= inv_d;
+        for (int e = 1; e < P; ++e) z = add2(z, g[e]);
+        float two[2] = {s.x + s.y, z.x + z.y};
+        reduce.sum(two);
+        return make_float2(two[0] * inv_d, two[1] * inv_d);
+    }
+    float one[1] = {s.x + s.y};
+    reduce.sum(one);
+    return make_float2(one[0] * inv_d, 0.0f);
 }
 
-// One block is one worker.  part[worker] holds, one behind the other, the sums of d_weight,
-// d_bias, d_post_weight, d_post_bias that exist.  Worker c and gate group g meet in slot c + g of
-// gate_part: along the rows one of the two grows by one at a time, so no two pairs share a slot.
+// part[block] holds, one behind the other, the sums of d_weight, d_bias, d_post_weight, d_post_bias
+// that exist; the teams of a block add theirs up first.  Team c and gate group g meet in slot c + g
+// of gate_part: along the rows one of the two grows by one at a time, so no two pairs share a slot.
+// MOST: threads of the largest block, which sets the registers that a thread may have.
 // NEXT: the following norm's gradient takes part; OWN: the update has a norm or a gate of its own.
-template <typename TS, typename TU, typename TY, int VEC, int NV, int R, bool FULL, bool NEXT, bool OWN>
-__global__ void __launch_bounds__(MAX_THREADS) join_bwd_kernel(const JoinArgs a) {
-    __shared__ __align__(16) float buffer[2 * MAX_WARPS * 4];
+// SHARED: the parameters are held in shared memory.
+template <typename TS, typename TU, typename TY, int VEC, int NV, int MOST, bool SHARED, bool FULL, bool NEXT, bool OWN>
+__global__ void __launch_bounds__(MOST) join_bwd_kernel(const JoinArgs a) {
+    __shared__ __align__(16) float buffer[REDUCER_FLOATS];
     using L = Lane<VEC, NV>;
     constexpr int P = L::P;
     const L lane(a.d);
+    const bool owner = team_of_grid() < a.owners;
+    const long long lo = owner ? first_row(team_of_grid(), a.rows, a.owners) : 0;
+    const long long hi = owner ? first_row(team_of_grid() + 1LL, a.rows, a.owners) : 0;
     using FS = Feed<TS, VEC, NV>;
     using FU = Feed<TU, VEC, NV>;
     using FY = Feed<TY, VEC, NV>;
     FS from_grad, from_stream;
     FU from_update;
     FY from_normed;
-    constexpr int BYTES = FS::BYTES + (NEXT ? FS::BYTES + FY::BYTES : 0) + (OWN ? FU::BYTES : 0);
-    const uint32_t per_slot = BYTES * blockDim.x;
-    uint32_t region = (uint32_t)__cvta_generic_to_shared(join_shared);
-    from_grad.place(a.d_stream, a.d, region);
+    const uint32_t per_slot = (FS::BYTES + (NEXT ? FS::BYTES + FY::BYTES : 0) + (OWN ? FU::BYTES : 0)) * blockDim.x;
+    using H = Held<VEC, NV, SHARED>;
+    const uint32_t held_bytes = H::BYTES * blockDim.x;
+    constexpr int HELD = (NEXT ? 1 : 0) + (OWN ? (FULL ? 2 : 1) : 0);
+    // the teams' columns are the same: they share the parameters, and each has its gate and slots
+    uint32_t held_at = (uint32_t)__cvta_generic_to_shared(join_shared);
+    const uint32_t gate_at = held_at + HELD * held_bytes + threadIdx.y * (a.slots * per_slot + (OWN ? held_bytes : 0));
+    uint32_t region = gate_at + (OWN ? held_bytes : 0);
+    from_grad.open(a.d_stream, a.d, lo, region);
     region += FS::BYTES * blockDim.x;
     if (NEXT) {
-        from_stream.place(a.stream, a.d, region);
+        from_stream.open(a.stream, a.d, lo, region);
         region += FS::BYTES * blockDim.x;
-        from_normed.place(a.d_normed, a.d, region);
+        from_normed.open(a.d_normed, a.d, lo, region);
         region += FY::BYTES * blockDim.x;
     }
-    if (OWN) from_update.place(a.update, a.update_stride, region);
-    Walk<R> walk(a);
-    auto fetch = [&](long long row, int slot) {
-        const uint32_t at = slot * per_slot;
-        if (a.d_stream) from_grad.fetch(lane, row, at);
+    if (OWN) from_update.open(a.update, a.update_stride, lo, region);
+    auto fetch = [&](uint32_t at, bool exists) {
         if (NEXT) {
-            from_stream.fetch(lane, row, at);
-            from_normed.fetch(lane, row, at);
+            from_normed.fetch(lane, at, exists);
+            from_stream.fetch(lane, at, exists);
         }
-        if (OWN) from_update.fetch(lane, row, at);
+        from_grad.fetch(lane, at, exists && a.d_stream);
+        if (OWN) from_update.fetch(lane, at, exists);
+        feed_commit();
     };
-    walk.ahead(walk.slots, fetch);
+    for (int i = 0; i < a.slots; ++i) fetch(i * per_slot, lo + i < hi);
+    Sink<TS, VEC, NV> to_residual;
+    Sink<TU, VEC, NV> to_update;
+    to_residual.open(a.d_residual, lo, a.d);
+    to_update.open(a.d_update, lo, a.d);
     Reducer reduce(buffer);
     const float inv_d = 1.0f / (float)a.d;
-    float2 w[P], pw[P], pb[P], gate[P];
+    Gate<VEC, NV, SHARED && OWN> gate(a, lo, gate_at);
+    H weight, post_weight, post_bias;
+    auto hold = [&](H& held, const void* p, float otherwise) {
+        float2 v[P];
+        lane.param(p, a.param_code, otherwise, v);
+        held.set(v, held_at);
+        held_at += held_bytes;
+    };
+    if (NEXT) hold(weight, a.weight, 1.0f);
+    if (OWN) hold(post_weight, a.post_weight, 1.0f);
+    if (OWN && FULL) hold(post_bias, a.post_bias, 0.0f);
     float2 dw[P], db[P], dpw[P], dpb[P], dg[P];
-    lane.param(a.weight, a.param_code, 1.0f, w);
-    lane.param(a.post_weight, a.param_code, 1.0f, pw);
-    lane.fill(a.scale, gate);
     lane.fill(0.0f, dw);
     lane.fill(0.0f, dpw);
     lane.fill(0.0f, dg);
-    if (FULL) {
-        lane.param(a.post_bias, a.param_code, 0.0f, pb);
-        lane.fill(0.0f, db);
-        lane.fill(0.0f, dpb);
-    }
-    // d_gate is gathered without the scale, which is put on where it is stored
-    auto flush = [&](long long group) {
+    lane.fill(0.0f, db);
+    lane.fill(0.0f, dpb);
+    auto flush = [&]() {                 // d_gate is gathered without the scale
         #pragma unroll
         for (int e = 0; e < P; ++e) dg[e] = mul2(dg[e], both(a.scale));
-        lane.store(a.gate_part + (blockIdx.x + group) * a.d, dg);
+        lane.store(a.gate_part + (team_of_grid() + gate.group) * a.d, dg);
         lane.fill(0.0f, dg);
     };
-    while (walk.row < walk.hi) {
-        const long long before = walk.group;
-        const bool fresh = walk.next();
-        if (OWN && fresh) {
-            if (before >= 0) flush(before);
-            lane.param(static_cast<const char*>(a.gate) + walk.group * a.d * param_bytes(a.gate_code), a.gate_code,
-                       1.0f, gate);
-            #pragma unroll
-            for (int e = 0; e < P; ++e) gate[e] = mul2(gate[e], both(a.scale));
+    uint32_t slot = 0;
+    const uint32_t last_slot = (a.slots - 1) * per_slot;
+    float4 coming = lo < hi ? a.stats[lo] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (long long row = lo; row < hi; ++row) {
+        if (OWN && row >= gate.end) {
+            if (gate.group >= 0) flush();
+            gate.move(a, lane, row);
         }
-        float4 st[R];
-        #pragma unroll
-        for (int i = 0; i < R; ++i) st[i] = i < walk.count ? a.stats[walk.row + i] : make_float4(0.f, 0.f, 0.f, 0.f);
-        feed_wait(walk.slots - R);
-        float2 dr[R][P], u[R][P];
-        #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            lane.fill(0.0f, dr[i]);
-            if (i < walk.count && a.d_stream) from_grad.get(lane, walk.row + i, walk.slot_of(i) * per_slot, dr[i]);
-        }
+        const float4 st = coming;
+        if (row + 1 < hi) coming = a.stats[row + 1];
+        feed_wait(a.slots - 1);
+        float2 dr[P], u[P];
         if (NEXT) {
-            float2 g[R][P], hat[R][P];
-            float m1[R], m0[R];
-            #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                lane.fill(0.0f, g[i]);
-                lane.fill(0.0f, hat[i]);
-                if (i < walk.count) {
-                    const uint32_t at = walk.slot_of(i) * per_slot;
-                    from_normed.get(lane, walk.row + i, at, g[i]);
-                    from_stream.get(lane, walk.row + i, at, hat[i]);
-                }
-            }
-            if (!OWN) walk.ahead(walk.count, fetch);
-            #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (FULL && a.layer) {
-                    #pragma unroll
-                    for (int e = 0; e < P; ++e) hat[i][e] = add2(hat[i][e], both(-st[i].z));
-                    lane.mask(hat[i]);
-                }
+            float2 g[P], hat[P];
+            from_normed.get(lane, slot, g);
+            from_stream.get(lane, slot, hat);
+            if (FULL && a.layer) {
                 #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    hat[i][e] = mul2(hat[i][e], both(st[i].w));
-                    dw[e] = fma2(g[i][e], hat[i][e], dw[e]);
-                    if (FULL) db[e] = add2(db[e], g[i][e]);
-                    g[i][e] = mul2(g[i][e], w[e]);
-                }
+                for (int e = 0; e < P; ++e) hat[e] = add2(hat[e], both(-st.z));
+                lane.mask(hat);
             }
-            backward_sums<FULL>(g, hat, a.layer, inv_d, reduce, m1, m0);
+            float2 w[P];
+            weight.get(w);
             #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const float2 rs = both(st[i].w), back = both(-m1[i] * st[i].w);
-                #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    if (FULL) g[i][e] = add2(g[i][e], both(-m0[i]));
-                    dr[i][e] = fma2(g[i][e], rs, fma2(hat[i][e], back, dr[i][e]));
-                }
-                if (FULL) lane.mask(dr[i]);
+            for (int e = 0; e < P; ++e) {
+                hat[e] = mul2(hat[e], both(st.w));
+                dw[e] = fma2(g[e], hat[e], dw[e]);
+                if (FULL) db[e] = add2(db[e], g[e]);
+                g[e] = mul2(g[e], w[e]);
             }
-        }
+            const float2 m = backward_means<FULL>(g, hat, a.layer, inv_d, reduce);
+            if (a.d_stream) from_grad.get(lane, slot, dr);
+            else lane.fill(0.0f, dr);
+            const float2 r = both(st.w), back = both(-m.x * st.w);
+            #pragma unroll
+            for (int e = 0; e < P; ++e) {
+                if (FULL) g[e] = add2(g[e], both(-m.y));
+                dr[e] = fma2(g[e], r, fma2(hat[e], back, dr[e]));
+            }
+            if (FULL) lane.mask(dr);
+        } else from_grad.get(lane, slot, dr);        // without a following norm there is a gradient here
+        if (OWN) from_update.get(lane, slot, u);
+        fetch(slot, row + a.slots < hi);
+        slot = slot == last_slot ? 0 : slot + per_slot;
+        if (a.d_residual) to_residual.put(lane, dr, a.d);
         if (OWN) {
-            #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                lane.fill(0.0f, u[i]);
-                if (i < walk.count) from_update.get(lane, walk.row + i, walk.slot_of(i) * per_slot, u[i]);
-            }
-        }
-        if (OWN || !NEXT) walk.ahead(walk.count, fetch);
-        if (a.d_residual) {
-            #pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (i < walk.count) lane.store(static_cast<TS*>(a.d_residual) + (walk.row + i) * a.d, dr[i]);
-        }
-        if (OWN) {
-            #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (FULL && a.layer && a.post_weight) {
-                    #pragma unroll
-                    for (int e = 0; e < P; ++e) u[i][e] = add2(u[i][e], both(-st[i].x));
-                    lane.mask(u[i]);
-                }
+            if (FULL && a.layer && a.post_weight) {
                 #pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    u[i][e] = mul2(u[i][e], both(st[i].y));            // the update itself without a post norm
-                    const float2 v = FULL ? fma2(u[i][e], pw[e], pb[e]) : mul2(u[i][e], pw[e]);
-                    dg[e] = fma2(dr[i][e], v, dg[e]);
-                    dr[i][e] = mul2(dr[i][e], gate[e]);
-                    dpw[e] = fma2(dr[i][e], u[i][e], dpw[e]);
-                    if (FULL) dpb[e] = add2(dpb[e], dr[i][e]);
-                    dr[i][e] = mul2(dr[i][e], pw[e]);
-                }
+                for (int e = 0; e < P; ++e) u[e] = add2(u[e], both(-st.x));
+                lane.mask(u);
+            }
+            float2 pw[P], pb[P], gv[P];
+            post_weight.get(pw);
+            if (FULL) post_bias.get(pb);
+            gate.held.get(gv);
+            #pragma unroll
+            for (int e = 0; e < P; ++e) {
+                u[e] = mul2(u[e], both(st.y));            // the update itself without a post norm
+                const float2 v = FULL ? fma2(u[e], pw[e], pb[e]) : mul2(u[e], pw[e]);
+                dg[e] = fma2(dr[e], v, dg[e]);
+                dr[e] = mul2(dr[e], gv[e]);
+                dpw[e] = fma2(dr[e], u[e], dpw[e]);
+                if (FULL) dpb[e] = add2(dpb[e], dr[e]);
+                dr[e] = mul2(dr[e], pw[e]);
             }
             if (a.post_weight) {
-                float m1[R], m0[R];
-                backward_sums<FULL>(dr, u, a.layer, inv_d, reduce, m1, m0);
+                const float2 m = backward_means<FULL>(dr, u, a.layer, inv_d, reduce);
                 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    #pragma unroll
-                    for (int e = 0; e < P; ++e) {
-                        if (FULL) dr[i][e] = add2(dr[i][e], both(-m0[i]));
-                        dr[i][e] = mul2(both(st[i].y), fma2(u[i][e], both(-m1[i]), dr[i][e]));
-                    }
+                for (int e = 0; e < P; ++e) {
+                    if (FULL) dr[e] = add2(dr[e], both(-m.y));
+                    dr[e] = mul2(both(st.y), fma2(u[e], both(-m.x), dr[e]));
                 }
             }
         } else {
             #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                #pragma unroll
-                for (int e = 0; e < P; ++e) dr[i][e] = mul2(dr[i][e], gate[e]);
-            }
+            for (int e = 0; e < P; ++e) dr[e] = mul2(dr[e], both(a.scale));
         }
-        #pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (i < walk.count) lane.store(static_cast<TU*>(a.d_update) + (walk.row + i) * a.d, dr[i]);
-        walk.done();
+        to_update.put(lane, dr, a.d);
     }
-    if (OWN && a.gate && walk.group >= 0) flush(walk.group);
+    if (OWN && a.gate && gate.group >= 0) flush();
     const int sums = (NEXT ? (a.bias ? 2 : 1) : 0) + (a.post_weight ? (a.post_bias ? 2 : 1) : 0);
     float* mine = a.part + (size_t)blockIdx.x * sums * a.d;
-    if (NEXT) { lane.store(mine, dw); mine += a.d; }
-    if (FULL && NEXT && a.bias) { lane.store(mine, db); mine += a.d; }
-    if (OWN && a.post_weight) { lane.store(mine, dpw); mine += a.d; }
-    if (FULL && OWN && a.post_weight && a.post_bias) lane.store(mine, dpb);
+    auto leave = [&](const float2 (&v)[P]) {
+        if (blockDim.y == 1) lane.store(mine, v);
+        else {                          // the slots are free now: a team's row of d floats each
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(join_shared);
+            __syncthreads();
+            Held<VEC, NV, true> place;          // thread by thread, as it is read below
+            place.set(v, at + threadIdx.y * place.BYTES * blockDim.x);
+            __syncthreads();
+            if (threadIdx.y == 0) {
+                float2 total[P], more[P];
+                #pragma unroll
+                for (int e = 0; e < P; ++e) total[e] = v[e];
+                for (int y = 1; y < blockDim.y; ++y) {
+                    place.place = at + y * place.BYTES * blockDim.x + threadIdx.x * place.PIECE;
+                    place.get(more);
+                    #pragma unroll
+                    for (int e = 0; e < P; ++e) total[e] = add2(total[e], more[e]);
+                }
+                lane.store(mine, total);
+            }
+        }
+        mine += a.d;
+    };
+    if (blockDim.y > 1) asm volatile("cp.async.wait_all;" ::: "memory");
+    if (NEXT) leave(dw);
+    if (FULL && NEXT && a.bias) leave(db);
+    if (OWN && a.post_weight) leave(dpw);
+    if (FULL && OWN && a.post_weight && a.post_bias) leave(dpb);
 }
 
 struct SumArgs {
@@ -662,32 +719,36 @@ struct SumArgs {
     const float* gate_part;
     void* out[4];                      // one for each sum, in the order of part
     void* gate_out;                    // [groups][d]
-    long long rows, group_rows, groups, workers;
+    long long rows, group_rows, groups;
+    int blocks, owners;                // rows of part, teams that own rows
     int d, sums, param_code, gate_code;
 };
 
-// Column sums of the partial results: 32 columns a block, SLICES threads share a column, four
-// partial results under way in each.
-constexpr int SLICES = 32;
-__global__ void __launch_bounds__(32 * SLICES) join_sum_kernel(const SumArgs a) {
-    const int col = blockIdx.y * 32 + threadIdx.x;
+// Column sums of the partial results.  A block takes eight columns, one 32-byte sector of a partial
+// row, and SLICES threads share a column, four partial results under way in each: there are more
+// blocks than SMs even for one parameter of 1200 columns.
+constexpr int SLICES = 64;
+__global__ void __launch_bounds__(8 * SLICES) join_sum_kernel(const SumArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");           // the partial results are there
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
+    const int col = blockIdx.y * 8 + x;
     const long long which = blockIdx.x;
     const float* base;
-    long long lo = 0, hi = a.workers;
+    long long lo = 0, hi = a.blocks;
     size_t stride;
     if (which < a.sums) {
         base = a.part + which * a.d;
         stride = (size_t)a.sums * a.d;
     } else {
         const long long g = which - a.sums;
-        lo = owner_of(g * a.group_rows, a.rows, a.workers);
-        hi = owner_of((g + 1) * a.group_rows - 1, a.rows, a.workers) + 1;
+        lo = owner_of(g * a.group_rows, a.rows, a.owners);
+        hi = owner_of((g + 1) * a.group_rows - 1, a.rows, a.owners) + 1;
         base = a.gate_part + g * a.d;
         stride = a.d;
     }
     float acc = 0.0f;
     if (col < a.d) {
-        long long c = lo + threadIdx.y;
+        long long c = lo + y;
         for (; c + 3 * SLICES < hi; c += 4 * SLICES) {
             float v[4];
             #pragma unroll
@@ -697,89 +758,127 @@ __global__ void __launch_bounds__(32 * SLICES) join_sum_kernel(const SumArgs a) 
         }
         for (; c < hi; c += SLICES) acc += base[c * stride + col];
     }
-    __shared__ float slice[SLICES][33];
-    slice[threadIdx.y][threadIdx.x] = acc;
+    acc += __shfl_xor_sync(0xffffffffu, acc, 8);                 // four slices a warp
+    acc += __shfl_xor_sync(0xffffffffu, acc, 16);
+    __shared__ float slice[SLICES / 4][8];
+    if ((threadIdx.x & 31) < 8) slice[threadIdx.x >> 5][x] = acc;
     __syncthreads();
-    // warp y sums column y of the block
-    const float total = gb_warp_sum(slice[threadIdx.x][threadIdx.y]);
-    const int mine = blockIdx.y * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && mine < a.d) {
-        if (which < a.sums) gb_write(a.out[which], a.param_code, mine, total);
-        else gb_write(a.gate_out, a.gate_code, (size_t)(which - a.sums) * a.d + mine, total);
+    if (threadIdx.x < 8 && col < a.d) {
+        float total = slice[0][x];
+        #pragma unroll
+        for (int s = 1; s < SLICES / 4; ++s) total += slice[s][x];
+        if (which < a.sums) gb_write(a.out[which], a.param_code, col, total);
+        else gb_write(a.gate_out, a.gate_code, (size_t)(which - a.sums) * a.d + col, total);
     }
 }
 
 constexpr int MAX_WIDTH = 8192;
 
-// Threads of a block for rows of d values in vectors of vec, and its rounds of vectors: a single
-// round of eight columns a thread up to 4096 columns, two from there on; single values in up to
-// four rounds of 256 threads, then sixteen of 512.
-struct Shape { int threads, rounds; };
-Shape shape_of(int d, int vec) {
-    const int vectors = (d + vec - 1) / vec, most = vec == 8 || vectors > 1024 ? MAX_THREADS : 256;
-    int t = (vectors + 31) / 32 * 32;
-    if (t > most) t = most;
-    return Shape{t, (vectors + t - 1) / t};
+// How rows of d values in vectors of vec are dealt out: threads of a team, teams of a block, rounds
+// of vectors a thread.  Eight columns a thread up to 256, then 16 or 24: what a row costs beside
+// its values (addresses, the reduction) is shared by more of them.  Up to 768 columns a row is a
+// warp's, without a barrier.  Single values: up to four rounds of 256 threads, then sixteen of 512.
+// A block has as many teams as its registers allow (128 a thread forward, 168 backward up to 4096
+// columns), fewer where there are not rows enough for every SM.
+struct Shape { int threads, teams, rounds; };
+Shape shape_of(long long rows, int d, int vec, bool forward) {
+    const int vectors = (d + vec - 1) / vec;
+    Shape s{0, 1, 1};
+    if (vec == 8) {
+        s.rounds = vectors <= 96 ? (vectors + 31) / 32 : 2;
+        s.threads = vectors <= 96 ? 32 : ((vectors + 1) / 2 + 31) / 32 * 32;
+    } else {
+        const int most = vectors > 1024 ? MAX_THREADS : 256;
+        s.threads = (vectors + 31) / 32 * 32;
+        if (s.threads > most) s.threads = most;
+        s.rounds = (vectors + s.threads - 1) / s.threads;
+    }
+    const int most = (forward && s.rounds != 3) || s.threads > 384 ? 512 : 384;
+    const long long enough = (rows + 147) / 148;
+    s.teams = most / s.threads;
+    if (s.teams > 15) s.teams = 15;                  // a barrier each, and one for all
+    if (s.teams > enough) s.teams = (int)enough;
+    if (s.teams < 1) s.teams = 1;
+    return s;
+}
+int blocks_for(long long rows, const Shape& s) {
+    const long long want = (rows + s.teams - 1) / s.teams;
+    return (int)(want < 148 ? want : 148);
+}
+int owners_for(long long rows, const Shape& s) {
+    const long long teams = (long long)blocks_for(rows, s) * s.teams;
+    return (int)(rows < teams ? rows : teams);
 }
 
-// Blocks an SM holds at the 128 registers that 512 threads may have; each leaves a row of partial
-// sums, so there are no more than fill the SMs.
-int blocks_per_sm(int threads) {
-    const int n = 512 / threads;
-    return n < 1 ? 1 : n > 8 ? 8 : n;
-}
+constexpr int MAX_SHARED = 225 << 10;
 
-int workers_for(long long rows, int threads) {
-    const long long most = 148LL * blocks_per_sm(threads);
-    return (int)(rows < most ? rows : most);
-}
-
-// Slots that fit beside one another in an SM's 227 KB.
-int slots_for(int bytes_per_slot, int blocks, int rows_at_once) {
-    int n = bytes_per_slot ? (int)((220 << 10) / blocks / bytes_per_slot) : MAX_SLOTS;
-    return n < rows_at_once ? rows_at_once : n > MAX_SLOTS ? MAX_SLOTS : n;
-}
-
+// A launch with as many slots as fit in an SM.  `common` bytes a thread are the teams' together,
+// `own` each team's, beside `slot` for every slot.
 template <typename K>
-int start(K kernel, int grid, int threads, int bytes_per_slot, int blocks, int rows_at_once, JoinArgs a, cudaStream_t s) {
-    a.slots = slots_for(bytes_per_slot, blocks, rows_at_once);
-    const int shared = a.slots * bytes_per_slot;
+int start(K kernel, const Shape& shape, int slot, int common, int own, int add, JoinArgs a, cudaStream_t s) {
+    const int room = (MAX_SHARED - common * shape.threads) / shape.teams - own * shape.threads;
+    a.slots = slot ? room / (slot * shape.threads) : MAX_SLOTS;
+    if (a.slots > MAX_SLOTS) a.slots = MAX_SLOTS;
+    if (a.slots < 1) a.slots = 1;
+    int shared = ((a.slots * slot + own) * shape.teams + common) * shape.threads;
+    const int sums = shape.teams > 1 ? shape.teams * add * shape.threads : 0;          // where the teams add up
+    if (shared < sums) shared = sums;
     if (shared > (40 << 10)) {                       // more than a launch may take unasked, with the static part
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
         if (err != cudaSuccess) return (int)err;
     }
-    kernel<<<grid, threads, shared, s>>>(a);
+    a.owners = owners_for(a.rows, shape);
+    kernel<<<blocks_for(a.rows, shape), dim3(shape.threads, shape.teams), shared, s>>>(a);
     return (int)cudaGetLastError();
 }
 
-template <typename TS, typename TU, typename TY, int VEC, int NV, int R, bool FULL>
-int launch_form(bool forward, int threads, const JoinArgs& a, cudaStream_t s) {
+template <typename TS, typename TU, typename TY, int VEC, int NV, int MOST, bool FULL, bool SHARED>
+int launch_backward(const Shape& shape, const JoinArgs& a, cudaStream_t s) {
     constexpr int S = Feed<TS, VEC, NV>::BYTES, U = Feed<TU, VEC, NV>::BYTES, Y = Feed<TY, VEC, NV>::BYTES;
-    const int blocks = blocks_per_sm(threads);
-    const int grid = workers_for(a.rows, threads);
-    if (forward) return start(join_fwd_kernel<TS, TU, TY, VEC, NV, R, FULL>, grid, threads, (S + U) * threads, blocks, R, a, s);
+    constexpr int H = Held<VEC, NV, SHARED>::BYTES, A = Held<VEC, NV, true>::BYTES, O = FULL ? 2 : 1;
     const bool next = a.d_normed, own = a.post_weight || a.gate;
-    if (next && own) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, R, FULL, true, true>, grid, threads, (2 * S + Y + U) * threads, blocks, R, a, s);
-    if (next) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, R, FULL, true, false>, grid, threads, (2 * S + Y) * threads, blocks, R, a, s);
-    return start(join_bwd_kernel<TS, TU, TY, VEC, NV, R, FULL, false, true>, grid, threads, (S + U) * threads, blocks, R, a, s);
+    if (next && own) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, MOST, SHARED, FULL, true, true>, shape, 2 * S + Y + U, (1 + O) * H, H, A, a, s);
+    if (next) return start(join_bwd_kernel<TS, TU, TY, VEC, NV, MOST, SHARED, FULL, true, false>, shape, 2 * S + Y, H, 0, A, a, s);
+    return start(join_bwd_kernel<TS, TU, TY, VEC, NV, MOST, SHARED, FULL, false, true>, shape, S + U, O * H, H, A, a, s);
 }
 
-template <typename TS, typename TU, typename TY, int VEC, int NV, int R>
-int launch_shaped(bool forward, int threads, const JoinArgs& a, cudaStream_t s) {
-    if (a.layer || a.bias || a.post_bias) return launch_form<TS, TU, TY, VEC, NV, R, true>(forward, threads, a, s);
-    return launch_form<TS, TU, TY, VEC, NV, R, false>(forward, threads, a, s);
+template <typename TS, typename TU, typename TY, int VEC, int NV, int MOST, bool FULL>
+int launch_form(bool forward, const Shape& shape, const JoinArgs& a, cudaStream_t s) {
+    constexpr int S = Feed<TS, VEC, NV>::BYTES, U = Feed<TU, VEC, NV>::BYTES, Y = Feed<TY, VEC, NV>::BYTES;
+    if (forward) {
+        constexpr int H = Held<VEC, NV, (FULL && VEC * NV > 8 && NV < 16)>::BYTES;
+        return start(join_fwd_kernel<TS, TU, TY, VEC, NV, FULL>, shape, S + U, 4 * H, H, 0, a, s);
+    }
+    if constexpr (VEC * NV == 1) return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, false>(shape, a, s);
+    else {
+        // the widest rows with four parameters leave no room for a slot: registers hold them
+        if constexpr (MOST == 512 && FULL) {
+            constexpr int H = Held<VEC, NV, true>::BYTES;
+            if ((4 * H + 2 * S + Y + U) * shape.threads > MAX_SHARED)
+                return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, false>(shape, a, s);
+        }
+        return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, true>(shape, a, s);
+    }
+}
+
+template <typename TS, typename TU, typename TY, int VEC, int NV, int MOST>
+int launch_shaped(bool forward, const Shape& shape, const JoinArgs& a, cudaStream_t s) {
+    if (a.layer || a.bias || a.post_bias) return launch_form<TS, TU, TY, VEC, NV, MOST, true>(forward, shape, a, s);
+    return launch_form<TS, TU, TY, VEC, NV, MOST, false>(forward, shape, a, s);
 }
 
 template <typename TS, typename TU, typename TY>
 int launch(bool forward, int vec, const JoinArgs& a, cudaStream_t s) {
-    const Shape shape = shape_of(a.d, vec);
+    const Shape shape = shape_of(a.rows, a.d, vec, forward);
     if (vec == 8) {
-        if (shape.rounds == 1) return launch_shaped<TS, TU, TY, 8, 1, 2>(forward, shape.threads, a, s);
-        return launch_shaped<TS, TU, TY, 8, 2, 1>(forward, shape.threads, a, s);
+        if (shape.rounds == 1) return launch_shaped<TS, TU, TY, 8, 1, 384>(forward, shape, a, s);
+        if (shape.rounds == 3) return launch_shaped<TS, TU, TY, 8, 3, 384>(forward, shape, a, s);
+        if (shape.threads * shape.teams <= 384) return launch_shaped<TS, TU, TY, 8, 2, 384>(forward, shape, a, s);
+        return launch_shaped<TS, TU, TY, 8, 2, 512>(forward, shape, a, s);
     }
-    if (shape.rounds <= 1) return launch_shaped<TS, TU, TY, 1, 1, 2>(forward, shape.threads, a, s);
-    if (shape.rounds <= 4) return launch_shaped<TS, TU, TY, 1, 4, 2>(forward, shape.threads, a, s);
-    return launch_shaped<TS, TU, TY, 1, 16, 1>(forward, shape.threads, a, s);
+    if (shape.rounds <= 1) return launch_shaped<TS, TU, TY, 1, 1, 384>(forward, shape, a, s);
+    if (shape.rounds <= 4) return launch_shaped<TS, TU, TY, 1, 4, 384>(forward, shape, a, s);
+    return launch_shaped<TS, TU, TY, 1, 16, 512>(forward, shape, a, s);
 }
 
 int dispatch(bool forward, int s, int u, int y, int vec, const JoinArgs& a, cudaStream_t stream) {
@@ -815,10 +914,12 @@ extern "C" int gb_residual_norm_fwd(int s, int u, int y, int vec, const void* re
     return dispatch(true, s, u, y, vec, a, cuda_stream);
 }
 
-// Workers (blocks) of a backward call: part holds workers * sums * d floats, gate_part
-// (workers + groups - 1) * d.
-extern "C" int gb_residual_norm_workers(long long rows, int d, int vec) {
-    return workers_for(rows, shape_of(d, vec).threads);
+// Blocks of a backward call and teams of them that own rows: part holds blocks * sums * d floats,
+// gate_part (owners + groups - 1) * d.
+extern "C" void gb_residual_norm_workers(long long rows, int d, int vec, int* blocks, int* owners) {
+    const Shape s = shape_of(rows, d, vec, false);
+    *blocks = blocks_for(rows, s);
+    *owners = owners_for(rows, s);
 }
 
 // The stream, both gradients (either may be null) and the outputs are [rows, d] without gaps;
@@ -845,12 +946,21 @@ extern "C" int gb_residual_norm_bwd(int s, int u, int y, int vec, const void* d_
     q.part = part; q.gate_part = gate_part; q.gate_out = gate_out;
     q.out[0] = out0; q.out[1] = out1; q.out[2] = out2; q.out[3] = out3;
     q.rows = rows; q.group_rows = group_rows; q.groups = gate ? rows / group_rows : 0;
-    q.workers = gb_residual_norm_workers(rows, d, vec);
+    gb_residual_norm_workers(rows, d, vec, &q.blocks, &q.owners);
     q.d = d; q.param_code = param_code; q.gate_code = gate_code;
     q.sums = (d_normed ? (bias ? 2 : 1) : 0) + (post_weight ? (post_bias ? 2 : 1) : 0);
     const long long what = q.sums + q.groups;
     if (what == 0) return 0;
     if (what > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    join_sum_kernel<<<dim3((unsigned)what, (d + 31) / 32), dim3(32, SLICES), 0, cuda_stream>>>(q);
-    return (int)cudaGetLastError();
+    // its blocks may be set up while the last of the gradients are on their way
+    cudaLaunchAttribute overlap = {};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)what, (d + 7) / 8);
+    config.blockDim = dim3(8 * SLICES);
+    config.stream = cuda_stream;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&config, join_sum_kernel, q);
 }

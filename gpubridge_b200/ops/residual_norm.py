@@ -41,7 +41,8 @@ def _declare(lib):
     vp, i, f, lg = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
     lib.gb_residual_norm_fwd.argtypes = [i, i, i, i, vp, lg, vp, lg, vp, vp, vp, vp, vp, vp, vp, i, vp, i,
                                          lg, lg, i, i, f, f, vp]
-    lib.gb_residual_norm_workers.argtypes = [lg, i, i]
+    lib.gb_residual_norm_workers.argtypes = [lg, i, i, ctypes.POINTER(i), ctypes.POINTER(i)]
+    lib.gb_residual_norm_workers.restype = None
     lib.gb_residual_norm_bwd.argtypes = [i, i, i, i, vp, vp, vp, vp, lg, vp, vp, vp, vp, vp, i, vp, i, vp, vp,
                                          vp, vp, vp, vp, vp, vp, vp, lg, lg, i, i, f, vp]
     lib._residual_norm_declared = True
@@ -124,11 +125,12 @@ class _ResidualNorm(torch.autograd.Function):
         if rows:
             vec = 8 if _aligned(d, u2, *(None if g is None else g.view(-1, d) for g in given)) else 1
             lib = _declare(_lib.lib())
-            workers = lib.gb_residual_norm_workers(rows, d, vec)
+            blocks, owners = ctypes.c_int(), ctypes.c_int()
+            lib.gb_residual_norm_workers(rows, d, vec, blocks, owners)
             sums = [t for t in outs if t is not None]
-            part = torch.empty(workers * len(sums) * d, dtype=torch.float32, device=device)
+            part = torch.empty(blocks.value * len(sums) * d, dtype=torch.float32, device=device)
             gate_part = (None if gate is None else
-                         torch.empty((workers + groups - 1) * d, dtype=torch.float32, device=device))
+                         torch.empty((owners.value + groups - 1) * d, dtype=torch.float32, device=device))
             slots = [t.data_ptr() for t in sums] + [None] * (4 - len(sums))
             with torch.cuda.device(device):
                 _lib.check(lib.gb_residual_norm_bwd(
