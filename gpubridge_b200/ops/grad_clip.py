@@ -13,33 +13,15 @@ On CPU tensors the same results come from plain torch operations.
 """
 from __future__ import annotations
 
-import ctypes
 import math
-from collections.abc import Iterable, Sequence
+from collections.abc import Iterable
 
 import torch
 
-from gpubridge_b200.ops import _lib
+from gpubridge_b200.ops import _build_ops
 
-launches = 0
-_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _EPS = 1e-6
-
-
-def _declare(lib):
-    if getattr(lib, "_grad_clip_declared", False):
-        return lib
-    vp, i, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_double
-    table, sizes = ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_longlong)
-    lib.gb_grad_norm_parts.argtypes = [table, sizes, i]
-    lib.gb_grad_norm_partial.argtypes = [i, i, table, sizes, i, vp, vp]
-    lib.gb_grad_norm_finish.argtypes = [i, vp, i, d, d, vp, vp]
-    lib.gb_grad_clip_coef.argtypes = [vp, d, vp, vp]
-    lib.gb_grad_scale.argtypes = [i, table, sizes, i, vp, vp]
-    lib.gb_adamw_clipped.argtypes = [vp, vp, vp, vp, ctypes.c_size_t, vp, d, d, d, d, d,
-                                     ctypes.c_float, vp, i, vp]
-    lib._grad_clip_declared = True
-    return lib
 
 
 def _norm_type(value) -> bool:
@@ -72,7 +54,7 @@ def _checked(tensors) -> tuple[list[torch.Tensor], torch.device | None]:
         if hasattr(t, "to_local"):
             raise TypeError("a DTensor's norm spans ranks: pass its local parts and join their norms, "
                             "or use torch.nn.utils.clip_grad_norm_")
-        if t.dtype not in _CODES and not (t.device.type == "cpu" and t.is_floating_point()):
+        if t.dtype not in _FLOATS and not (t.device.type == "cpu" and t.is_floating_point()):
             raise ValueError(f"gradients are float32, bfloat16 or float16 on the GPU, got {t.dtype}")
         if device is None:
             device = t.device
@@ -95,21 +77,6 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _groups(tensors: Sequence[torch.Tensor]):
-    """(type code, pointer table, size table, count) of each launch: one type, at most as many
-    tensors as a launch carries."""
-    most = _lib.lib().gb_grad_norm_max_tensors()
-    by_type: dict[torch.dtype, list[torch.Tensor]] = {}
-    for t in tensors:
-        if t.numel():
-            by_type.setdefault(t.dtype, []).append(t)
-    for dtype, members in by_type.items():
-        for lo in range(0, len(members), most):
-            part = members[lo:lo + most]
-            yield (_CODES[dtype], (ctypes.c_void_p * len(part))(*[t.data_ptr() for t in part]),
-                   (ctypes.c_longlong * len(part))(*[t.numel() for t in part]), len(part))
-
-
 def _cpu_norm(tensors, maximum: bool, scale: float = 1.0) -> torch.Tensor:
     if maximum:
         parts = [t.abs().max().double() for t in tensors if t.numel()]
@@ -120,26 +87,12 @@ def _cpu_norm(tensors, maximum: bool, scale: float = 1.0) -> torch.Tensor:
     return (total * abs(scale)).float()
 
 
-def _gpu_norm(tensors, device, maximum: bool, max_norm: float, scale: float = 1.0) -> torch.Tensor:
-    """Device tensor of two floats: the norm times ``|scale|``, and the factor that clips it."""
-    global launches
-    lib = _declare(_lib.lib())
-    with torch.cuda.device(device):
-        kept = [t if _dense(t) else t.contiguous() for t in tensors]
-        groups = list(_groups(kept))
-        counts = [lib.gb_grad_norm_parts(table, sizes, n) for _, table, sizes, n in groups]
-        if any(c < 0 for c in counts):
-            raise ValueError("too many gradient values for one call")
-        part = torch.empty(max(1, sum(counts)), dtype=torch.float64, device=device)
-        result = torch.empty(2, dtype=torch.float32, device=device)
-        stream, at = _lib.stream_ptr(device), 0
-        for (code, table, sizes, n), count in zip(groups, counts):
-            _lib.check(lib.gb_grad_norm_partial(code, int(maximum), table, sizes, n,
-                                                part.data_ptr() + 8 * at, stream), "gb_grad_norm_partial")
-            at += count
-        _lib.check(lib.gb_grad_norm_finish(int(maximum), part.data_ptr(), at, float(scale), max_norm,
-                                           result.data_ptr(), stream), "gb_grad_norm_finish")
-    launches += len(groups) + 1
+def _gpu_norm(tensors, maximum: bool, max_norm: float) -> torch.Tensor:
+    """Device tensor of two floats: the norm, and the factor that clips it."""
+    ops = _build_ops.load()
+    result = ops.grad_norm(tensors, maximum, 1.0, max_norm)
+    if result is None:                         # gaps between the values, or a list without tensors
+        result = ops.grad_norm([t if _dense(t) else t.contiguous() for t in tensors], maximum, 1.0, max_norm)
     return result
 
 
@@ -147,11 +100,17 @@ def grad_norm(tensors: Iterable[torch.Tensor] | torch.Tensor, norm_type: float =
     """The 2-norm (or, with ``norm_type=inf``, the largest magnitude) over all values of
     ``tensors``, as a 0-dim float32 tensor on their device.  An empty list has norm 0."""
     maximum = _norm_type(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if tensors and isinstance(tensors[0], torch.Tensor) and tensors[0].is_cuda and \
+            all(isinstance(t, torch.Tensor) for t in tensors):
+        result = _build_ops.load().grad_norm(tensors, maximum, 1.0, 0.0)
+        if result is not None:
+            return result[0]
     tensors, device = _checked(tensors)
     with torch.no_grad():
         if device is None or device.type != "cuda":
             return _cpu_norm(tensors, maximum)
-        return _gpu_norm(tensors, device, maximum, 0.0)[0]
+        return _gpu_norm(tensors, maximum, 0.0)[0]
 
 
 def _refuse_overlap(tensors) -> None:
@@ -162,18 +121,11 @@ def _refuse_overlap(tensors) -> None:
             raise ValueError("two of the gradients share memory: it would be scaled twice")
 
 
-def _scale_(tensors, device, result: torch.Tensor) -> None:
-    global launches
-    lib = _declare(_lib.lib())
-    coef = result.data_ptr() + 4
-    with torch.cuda.device(device):
-        for code, table, sizes, n in _groups([t for t in tensors if _dense(t)]):
-            _lib.check(lib.gb_grad_scale(code, table, sizes, n, coef, _lib.stream_ptr(device)),
-                       "gb_grad_scale")
-            launches += 1
-        for t in tensors:
-            if not _dense(t):                  # gaps between the values: torch walks the strides
-                t.copy_(t.float() * result[1])
+def _scale_(tensors, result: torch.Tensor) -> None:
+    _build_ops.load().grad_scale([t for t in tensors if _dense(t)], result)
+    for t in tensors:
+        if not _dense(t):                      # gaps between the values: torch walks the strides
+            t.copy_(t.float() * result[1])
 
 
 def _grads(parameters) -> list[torch.Tensor]:
@@ -186,7 +138,6 @@ def clip_grads_with_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max
                           total_norm: torch.Tensor) -> None:
     """Scale the parameters' gradients, in place, by ``min(1, max_norm / (total_norm + 1e-6))`` for
     a norm found elsewhere (over shards on several ranks): a float32 scalar tensor on their device."""
-    global launches
     max_norm = _max_norm(max_norm)
     tensors, device = _checked(_grads(parameters))
     if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1 or total_norm.dtype != torch.float32:
@@ -202,13 +153,7 @@ def clip_grads_with_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max
             for t in tensors:
                 t.mul_(coef.to(t.dtype) if t.dtype == torch.float64 else coef)
             return
-        result = torch.empty(2, dtype=torch.float32, device=device)
-        with torch.cuda.device(device):
-            _lib.check(_declare(_lib.lib()).gb_grad_clip_coef(
-                total_norm.data_ptr(), max_norm, result.data_ptr(), _lib.stream_ptr(device)),
-                "gb_grad_clip_coef")
-        launches += 1
-        _scale_(tensors, device, result)
+        _scale_(tensors, _build_ops.load().grad_coef(total_norm.detach(), max_norm))
 
 
 def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm: float,
@@ -223,14 +168,14 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor] | torch.Tensor, max_norm:
     with torch.no_grad():
         on_gpu = device is not None and device.type == "cuda"
         if on_gpu:
-            result = _gpu_norm(tensors, device, maximum, max_norm)
+            result = _gpu_norm(tensors, maximum, max_norm)
             norm = result[0]
         else:
             norm = _cpu_norm(tensors, maximum)
         if error_if_nonfinite and not bool(torch.isfinite(norm)):
             raise RuntimeError(f"the gradients' norm is {float(norm)}: not clipped")
         if on_gpu:
-            _scale_(tensors, device, result)
+            _scale_(tensors, result)
         elif tensors:
             coef = (max_norm / (norm.double() + _EPS)).clamp(max=1.0).float()
             for t in tensors:

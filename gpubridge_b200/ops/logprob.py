@@ -16,17 +16,14 @@ fixed order.  On the CPU the same formulas run as plain torch operations.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from gpubridge_b200.ops import _lib
+from gpubridge_b200.ops import _build_ops
 
-launches = 0
-_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
 class PolicyLoss(NamedTuple):
@@ -40,175 +37,6 @@ class PreferenceLoss(NamedTuple):
     loss: torch.Tensor          # 0-dim, differentiable
     rewards: torch.Tensor       # [sequences]: beta * (logprob - reference)
     logprobs: torch.Tensor      # [sequences]: sum (or mean) over a sequence's tokens
-
-
-def _declare(lib):
-    if getattr(lib, "_logprob_declared", False):
-        return lib
-    vp, i, f, d, lg = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double, ctypes.c_longlong
-    rows = [i, vp, lg, lg, lg, lg, i, i, vp, f]
-    lib.gb_token_logprobs.argtypes = rows + [vp, vp, vp]
-    lib.gb_policy_loss.argtypes = rows + [vp, vp, vp, vp, vp, f, f, f, vp, vp, vp, vp, vp, vp, vp, vp, vp]
-    lib.gb_logprob_grad.argtypes = rows + [vp, vp, vp, vp, vp]
-    lib.gb_preference_loss.argtypes = [vp, vp, vp, lg, lg, i, i, i, vp, i, d, d, vp, vp, vp, vp, vp, vp, vp]
-    lib._logprob_declared = True
-    return lib
-
-
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
-
-
-class _Rows:
-    """The rows of a logits tensor as the kernels take them, and room for their gradient."""
-
-    def __init__(self, logits: torch.Tensor, vocab: int) -> None:
-        ld, step = logits.shape[-1], 16 // logits.element_size()
-        self.shape = logits.shape
-        strided = (logits.dim() in (2, 3) and (ld == 1 or logits.stride(-1) == 1) and ld % step == 0
-                   and logits.data_ptr() % 16 == 0 and all(s % step == 0 for s in logits.stride()[:-1]))
-        if not logits.is_contiguous() and not strided:
-            logits = logits.contiguous()
-        self.logits, self.rows = logits, logits.numel() // ld
-        if logits.is_contiguous():
-            batch, row, inner = 0, ld, max(1, self.rows)
-        elif logits.dim() == 2:
-            batch, row, inner = 0, logits.stride(0), max(1, self.rows)
-        else:
-            batch, row, inner = logits.stride(0), logits.stride(1), logits.shape[1]
-        self.skew = (logits.data_ptr() % 16) // logits.element_size()
-        self.head = (_CODES[logits.dtype], logits.data_ptr(), batch, row, inner, self.rows, vocab, ld)
-
-    def grad(self) -> torch.Tensor:
-        """[..., ld] without gaps, as far from a 16-byte boundary as the logits."""
-        like = self.logits
-        if not self.skew:
-            return torch.empty(self.shape, dtype=like.dtype, device=like.device)
-        room = torch.empty(like.numel() + self.skew, dtype=like.dtype, device=like.device)
-        return room[self.skew:].view(self.shape)
-
-
-def _grad(rows: _Rows, targets, temperature, stats, coef, upstream) -> torch.Tensor:
-    global launches
-    grad = rows.grad()
-    if rows.rows:
-        device = grad.device
-        with torch.cuda.device(device):
-            _lib.check(_declare(_lib.lib()).gb_logprob_grad(
-                *rows.head, targets.data_ptr(), temperature, stats.data_ptr(), coef.data_ptr(), _ptr(upstream),
-                grad.data_ptr(), _lib.stream_ptr(device)), "gb_logprob_grad")
-        launches += 1
-    return grad
-
-
-def _logprobs(rows: _Rows, targets, temperature, keep_stats: bool):
-    """(log-probabilities [rows], stats or None)."""
-    global launches
-    device = rows.logits.device
-    logprobs = torch.empty(targets.shape, dtype=torch.float32, device=device)
-    stats = torch.empty((rows.rows, 2), dtype=torch.float32, device=device) if keep_stats else None
-    if rows.rows:
-        with torch.cuda.device(device):
-            _lib.check(_declare(_lib.lib()).gb_token_logprobs(
-                *rows.head, targets.data_ptr(), temperature, logprobs.data_ptr(), _ptr(stats),
-                _lib.stream_ptr(device)), "gb_token_logprobs")
-        launches += 1
-    return logprobs, stats
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, vocab, temperature):
-        rows = _Rows(logits, vocab)
-        logprobs, stats = _logprobs(rows, targets, temperature, ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, targets, stats)
-        ctx.vocab, ctx.temperature = vocab, temperature
-        return logprobs
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_logprobs):
-        logits, targets, stats = ctx.saved_tensors
-        return _grad(_Rows(logits, ctx.vocab), targets, ctx.temperature, stats, d_logprobs.contiguous(), None), None, None, None
-
-
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, old, advantages, ref, weights, denominator, vocab, temperature, clip, kl_coef,
-                unit_grad):
-        global launches
-        rows, device = _Rows(logits, vocab), logits.device
-        n = rows.rows
-        needs = ctx.needs_input_grad[0]
-        grad = rows.grad() if needs and unit_grad else None
-        stats = torch.empty((n, 2), dtype=torch.float32, device=device) if needs and not unit_grad else None
-        logprobs = torch.empty(targets.shape, dtype=torch.float32, device=device)
-        scratch = torch.empty(4 * n + 1, dtype=torch.float32, device=device)
-        coef = scratch[3 * n + 1:]
-        loss, kl, clipped = out = tuple(torch.empty((), dtype=torch.float32, device=device) for _ in range(3))
-        if n:
-            with torch.cuda.device(device):
-                _lib.check(_declare(_lib.lib()).gb_policy_loss(
-                    *rows.head, targets.data_ptr(), temperature, old.data_ptr(), advantages.data_ptr(), _ptr(ref),
-                    _ptr(weights), _ptr(denominator), clip[0], clip[1], kl_coef, logprobs.data_ptr(), _ptr(stats),
-                    coef.data_ptr(), scratch.data_ptr(), *(t.data_ptr() for t in out), _ptr(grad),
-                    _lib.stream_ptr(device)),
-                    "gb_policy_loss")
-            launches += 2
-        else:
-            for t in out:
-                t.zero_()
-        ctx.grad = grad
-        if needs and not unit_grad:
-            ctx.save_for_backward(logits, targets, stats, coef)
-        ctx.unit_grad, ctx.vocab, ctx.temperature = unit_grad, vocab, temperature
-        ctx.mark_non_differentiable(logprobs, kl, clipped)
-        return loss, logprobs, kl, clipped
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss, *_):
-        if ctx.unit_grad:
-            if ctx.grad is None:
-                raise RuntimeError("policy_loss(unit_grad=True) hands its gradient out once: "
-                                   "leave unit_grad away for a second backward pass")
-            grad, ctx.grad = ctx.grad, None
-        else:
-            logits, targets, stats, coef = ctx.saved_tensors
-            grad = _grad(_Rows(logits, ctx.vocab), targets, ctx.temperature, stats, coef,
-                         d_loss.to(torch.float32).contiguous())
-        return (grad,) + (None,) * 11
-
-
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, ref, offsets, vocab, beta, smoothing, average):
-        global launches
-        rows, device = _Rows(logits, vocab), logits.device
-        n, sequences = rows.rows, ref.numel()
-        logprobs, stats = _logprobs(rows, targets, 1.0, ctx.needs_input_grad[0])
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        rewards, seq_logprobs, seq_coef = (torch.empty(sequences, dtype=torch.float32, device=device) for _ in range(3))
-        sums = torch.empty(sequences, dtype=torch.float64, device=device)
-        coef = torch.empty(n, dtype=torch.float32, device=device)
-        with torch.cuda.device(device):
-            _lib.check(_declare(_lib.lib()).gb_preference_loss(
-                logprobs.data_ptr(), targets.data_ptr(), _ptr(offsets), n, n // sequences, sequences, vocab,
-                int(average), ref.data_ptr(), int(ref.dtype == torch.float64), beta, smoothing, sums.data_ptr(),
-                seq_coef.data_ptr(), loss.data_ptr(), rewards.data_ptr(), seq_logprobs.data_ptr(),
-                coef.data_ptr(), _lib.stream_ptr(device)), "gb_preference_loss")
-        launches += 1
-        ctx.save_for_backward(logits, targets, stats, coef)
-        ctx.vocab = vocab
-        ctx.mark_non_differentiable(rewards, seq_logprobs)
-        return loss, rewards, seq_logprobs
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss, *_):
-        logits, targets, stats, coef = ctx.saved_tensors
-        grad = _grad(_Rows(logits, ctx.vocab), targets, 1.0, stats, coef, d_loss.to(torch.float32).contiguous())
-        return (grad,) + (None,) * 7
 
 
 # -- checks and the plain form ---------------------------------------------------------------------
@@ -227,8 +55,10 @@ def _check(logits, targets, vocab, temperature) -> tuple[torch.Tensor, int]:
         raise ValueError(f"vocab must be in [1, {logits.shape[-1]}], got {vocab}")
     if not (math.isfinite(temperature) and temperature > 0):
         raise ValueError(f"temperature must be positive, got {temperature}")
-    if logits.device.type == "cuda" and logits.dtype not in _CODES or not logits.is_floating_point():
+    if logits.is_cuda and logits.dtype not in _FLOATS or not logits.is_floating_point():
         raise ValueError(f"logits are float32, bfloat16 or float16 on the GPU, got {logits.dtype}")
+    if logits.is_cuda and (logits.layout is not torch.strided or hasattr(logits, "to_local")):
+        raise ValueError("logits are an ordinary strided tensor: not sparse and no DTensor")
     return targets.to(torch.int64).contiguous(), vocab
 
 
@@ -242,11 +72,12 @@ def _per_token(name, t, targets, like):
         raise ValueError(f"{name} is on {t.device}, targets on {targets.device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} takes no gradient: detach it")
-    try:
-        t = t.expand(targets.shape)
-    except RuntimeError:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, which does not broadcast to the targets' "
-                         f"{tuple(targets.shape)}") from None
+    if t.shape != targets.shape:
+        try:
+            t = t.expand(targets.shape)
+        except RuntimeError:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, which does not broadcast to the targets' "
+                             f"{tuple(targets.shape)}") from None
     wide = torch.float64 if like.dtype == torch.float64 else torch.float32
     return t.to(wide).contiguous()
 
@@ -267,9 +98,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, vocab: int | Non
     """``log softmax(logits[..., :vocab] / temperature)`` at ``targets``: float32 in the targets'
     shape, 0 where a target lies outside ``[0, vocab)``.  Differentiable in the logits."""
     targets, vocab = _check(logits, targets, vocab, temperature)
-    if logits.device.type != "cuda":
-        return _plain_logprobs(logits, targets, vocab, temperature)[0]
-    return _TokenLogprobs.apply(logits, targets, vocab, float(temperature))
+    if logits.is_cuda:
+        return _build_ops.load().token_logprobs(logits, targets, vocab, temperature)
+    return _plain_logprobs(logits, targets, vocab, temperature)[0]
 
 
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor,
@@ -310,9 +141,9 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
         if not isinstance(denominator, torch.Tensor) or denominator.numel() != 1 or denominator.device != logits.device:
             raise ValueError("denominator is a tensor of one value on the logits' device")
         denominator = denominator.detach().to(torch.float32).reshape(())
-    if logits.device.type == "cuda":
-        return PolicyLoss(*_PolicyLoss.apply(logits, targets, old, advantages, ref, weights, denominator, vocab,
-                                             float(temperature), (low, high), float(kl_coef), unit_grad))
+    if logits.is_cuda:
+        return PolicyLoss(*_build_ops.load().policy_loss(logits, targets, vocab, old, advantages, ref, weights,
+                                                         denominator, low, high, kl_coef, temperature, unit_grad))
     logprobs, counted = _plain_logprobs(logits, targets, vocab, temperature, weights)
     w = counted.to(logprobs.dtype) if weights is None else torch.where(counted, weights, torch.zeros_like(weights))
     total = w.double().sum() if denominator is None else denominator.double()
@@ -376,9 +207,9 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logprobs: t
                 raise ValueError(f"offsets must not fall and stay within the {targets.numel()} rows")
         offsets = offsets.to(logits.device).contiguous()
     ref_logprobs = ref_logprobs.contiguous()
-    if logits.device.type == "cuda":
-        return PreferenceLoss(*_PreferenceLoss.apply(logits, targets, ref_logprobs, offsets, vocab, beta,
-                                                     smoothing, bool(average)))
+    if logits.is_cuda:
+        return PreferenceLoss(*_build_ops.load().preference_loss(logits, targets, vocab, ref_logprobs, offsets, beta,
+                                                                 smoothing, average))
     logprobs, counted = _plain_logprobs(logits, targets, vocab, 1.0)
     if offsets is None:
         sums, tokens = logprobs.double().sum(1), counted.sum(1)

@@ -59,7 +59,6 @@ class FlatAdamW:
         launches += 1
 
     def _clipped_step(self, max_norm: float, grad_scale: float, zero_grad: bool) -> None:
-        global launches
         from gpubridge_b200.ops import grad_clip
         max_norm = grad_clip._max_norm(max_norm)
         if self.p.device.type != "cuda":
@@ -67,16 +66,11 @@ class FlatAdamW:
             coef = max_norm / (float(self.grad_norm) + 1e-6)
             self._reference_step(grad_scale * (1.0 if coef > 1.0 else coef), zero_grad)   # a NaN stays one
             return
-        result = grad_clip._gpu_norm([self.g], self.g.device, False, max_norm, grad_scale)
+        from gpubridge_b200.ops import _build_ops
+        result = _build_ops.load().adamw_clipped(
+            self.p, self.g, self.m, self.v, self.state, self.lr, self.betas[0], self.betas[1], self.eps,
+            self.weight_decay, grad_scale, max_norm, zero_grad)
         self.grad_norm = result[0]
-        with torch.cuda.device(self.p.device):
-            code = grad_clip._declare(_lib.lib()).gb_adamw_clipped(
-                self.p.data_ptr(), self.g.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
-                self.p.numel(), self.state.data_ptr(), self.lr, self.betas[0], self.betas[1], self.eps,
-                self.weight_decay, grad_scale, result.data_ptr() + 4, int(zero_grad),
-                _lib.stream_ptr(self.p.device))
-        _lib.check(code, "gb_adamw_clipped")
-        launches += 1
 
     def _reference_step(self, grad_scale: float, zero_grad: bool, lo: int = 0, hi: int | None = None,
                         last: bool = True) -> None:

@@ -216,8 +216,8 @@ class DataParallelTrainer:
     # -- the step --------------------------------------------------------------------------------
     def _own_kernels(self) -> int:
         """Launches of this library's kernels so far (every op module keeps a counter)."""
-        from gpubridge_b200.ops import grad_clip, layernorm, optim, xent
-        total = layernorm.launches + optim.launches + xent.launches + grad_clip.launches
+        from gpubridge_b200.ops import _build_ops, layernorm, optim, xent
+        total = layernorm.launches + optim.launches + xent.launches + _build_ops.launches()
         if self.fabric is not None:
             total += self.fabric.launches
         return total
