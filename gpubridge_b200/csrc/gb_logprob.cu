@@ -15,18 +15,29 @@
 // and sweeps it again out of L2 to write the gradient.  The preference loss needs whole sequences
 // first: forward reads the logits, backward reads them again and writes.
 //
-// A block owns a row.  A row may begin at any address: a vector that reaches over the row's end
-// is handled value by value, and a gradient's row lies across the vectors as the logits' row does.  Rows whose
-// target is outside the vocabulary, or whose weight is 0, are not read; their gradient is 0.
-// Row sums are in fp32 (a thread adds a few hundred terms in [0, 1], the block joins 512 of them),
-// sums over rows in 64 bits and in a fixed order.  Bound by memory.
-#include <math_constants.h>
+// A block owns a row, or a cluster where there are few.  A row may begin at any address: what lies
+// before its first whole vector and behind its last is handled value by value, and a gradient's row
+// lies across the vectors as the logits' row does.  Rows whose target is outside the vocabulary, or
+// whose weight is 0, are not read; their gradient is 0.  Row sums are in fp32 (a thread adds a few
+// hundred terms in [0, 1], the block joins 256 of them), sums over rows in 64 bits and in a fixed
+// order.
+//
+// Bound by memory, but closely followed by the instructions: a value costs one exponential a sweep
+// and about four others (packed maxima, packed fused multiply-adds).
+#include <cooperative_groups.h>
+#include <math.h>
 #include "gb_vec.cuh"
 
 namespace {
 
-constexpr int THREADS = 512;
-constexpr float LOG2E = 1.4426950408889634f;
+namespace cg = cooperative_groups;
+
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int BATCH = 4;                             // vectors of 16 bytes that a thread has under way
+// log2(e) in two parts: the rounding of one alone would shift every log-probability the same way
+// (by 1e-8 of the logits' spread, which a sum over a thousand tokens shows)
+constexpr float LOG2E = 1.4426950408889634f, LOG2E_REST = 1.9259629911266175e-8f;
 
 // 2^x by the special-function unit (2 ulp; below 2^-126 it gives 0, which no sum here resolves).
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -35,23 +46,97 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
-template <typename T> struct Pack16 {                 // 16 bytes
-    static constexpr int N = 16 / (int)sizeof(T);
-    uint4 q;
-    __device__ __forceinline__ void load(const T* p) { q = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void get(float (&v)[N]) const {
-        if constexpr (sizeof(T) == 4) {
-            v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y);
-            v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
-        } else {
-            Raw8<T> raw;
-            raw.q = q;
-            raw.get(v);
-        }
+// Two values in one instruction (sm_100a's packed fp32); each rounds as the single one does.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+          "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 exp2_2(float2 t) { return make_float2(fast_exp2(t.x), fast_exp2(t.y)); }
+
+// 16 bytes of values: their pairs, their maximum, and back.
+template <typename T> struct Pack;
+template <> struct Pack<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void pairs(const uint4& q, float2 (&v)[2]) {
+        v[0] = make_float2(__uint_as_float(q.x), __uint_as_float(q.y));
+        v[1] = make_float2(__uint_as_float(q.z), __uint_as_float(q.w));
     }
-    static __device__ __forceinline__ void store(T* p, const float (&v)[N]) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        else gb_store8(p, v);
+    template <int U> static __device__ __forceinline__ float top(const uint4 (&q)[U]) {
+        float m = -INFINITY;
+        #pragma unroll
+        for (int i = 0; i < U; ++i)
+            m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(q[i].x), __uint_as_float(q[i].y))),
+                      fmaxf(__uint_as_float(q[i].z), __uint_as_float(q[i].w)));
+        return m;
+    }
+    static __device__ __forceinline__ uint4 back(const float2 (&v)[2]) {
+        return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+    }
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void pairs(const uint4& q, float2 (&v)[4]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+    template <int U> static __device__ __forceinline__ float top(const uint4 (&q)[U]) {
+        __nv_bfloat162 m;
+        #pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q[i]);
+            const __nv_bfloat162 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            m = i ? __hmax2(m, a) : a;
+        }
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ uint4 back(const float2 (&v)[4]) {
+        uint4 q;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[i].x, v[i].y);
+        return q;
+    }
+};
+template <> struct Pack<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void pairs(const uint4& q, float2 (&v)[4]) {
+        const __half2* h = reinterpret_cast<const __half2*>(&q);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __half22float2(h[i]);
+    }
+    template <int U> static __device__ __forceinline__ float top(const uint4 (&q)[U]) {
+        __half2 m;
+        #pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const __half2* h = reinterpret_cast<const __half2*>(&q[i]);
+            const __half2 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            m = i ? __hmax2(m, a) : a;
+        }
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ uint4 back(const float2 (&v)[4]) {
+        uint4 q;
+        __half2* h = reinterpret_cast<__half2*>(&q);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[i].x, v[i].y);
+        return q;
     }
 };
 
@@ -61,169 +146,212 @@ struct Rows {
     long long batch_stride, row_stride, inner, rows;
     int vocab, ld;                       // columns that count, columns there are
     __device__ __forceinline__ long long offset(long long r) const {
+        if (inner == rows) return r * row_stride;
         const long long b = r / inner;
         return b * batch_stride + (r - b * inner) * row_stride;
     }
 };
 
-// A row in vectors: vector i holds the columns i * N - skew ...
+// A row, or one block's share of its whole vectors.  Vector i holds the columns i * N - skew and
+// on; the few columns before the first whole vector and behind the last are the edges.
 template <typename T>
 struct Row {
-    static constexpr int N = Pack16<T>::N;
-    const T* base;                       // 16-byte aligned, at or before the row's first value
-    int skew, vocab, full_lo, full_hi, vectors;   // [full_lo, full_hi): vectors wholly in the vocabulary
-    __device__ Row(const T* x, int vocab_) : vocab(vocab_) {
+    static constexpr int N = Pack<T>::N, P = N / 2;
+    const T* x;
+    const uint4* base;                   // at or before the row's first value
+    int skew, lo, hi;                    // this block's vectors
+    int head, tail, vocab;               // edges: columns [0, head) and [tail, vocab)
+    __device__ Row(const T* x_, int vocab_, int part, int parts) : x(x_), vocab(vocab_) {
         skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-        base = x - skew;
-        vectors = (vocab + skew + N - 1) / N;
-        full_lo = skew ? 1 : 0;
-        full_hi = (vocab + skew) / N;
+        base = reinterpret_cast<const uint4*>(x - skew);
+        int first = skew ? 1 : 0, last = (vocab + skew) / N;
+        if (last < first) last = first;
+        head = first * N - skew;
+        if (head > vocab) head = vocab;
+        if (!skew) head = 0;
+        tail = last * N - skew;
+        if (tail < head) tail = head;
+        if (tail > vocab) tail = vocab;
+        const int share = (last - first + parts - 1) / parts;
+        lo = first + part * share;
+        hi = lo + share;
+        if (lo > last) lo = last;
+        if (hi > last) hi = last;
     }
-    __device__ __forceinline__ bool full(int i) const { return i >= full_lo && i < full_hi; }
-    // any vector; columns outside the vocabulary read as -inf
-    __device__ __forceinline__ void load(int i, float (&v)[N]) const {
-        if (full(i)) {
-            Pack16<T> p;
-            p.load(base + (long long)i * N);
-            p.get(v);
-        } else {
-            #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int col = i * N - skew + j;
-                v[j] = (col >= 0 && col < vocab) ? gb_up(base[(long long)i * N + j]) : -CUDART_INF_F;
+    __device__ __forceinline__ int edges() const { return head + vocab - tail; }
+    __device__ __forceinline__ int edge(int i) const { return i < head ? i : tail + i - head; }
+};
+
+// Where x k leaves fp32: a row whose maximum is the type's lowest value (all of it masked), or inf.
+__device__ __forceinline__ bool is_far(float m, float k) { return !(fabsf(m) * k < 1e38f); }
+
+// Running maximum m and sum s of 2^(x k + c) with c near -m k: c is held instead of m k, so what
+// its rounding is does not matter.  The maximum of a batch decides whether the sum is rescaled,
+// which is rare after the first few.  While the maximum is far, nothing is summed that counts.
+struct Running {
+    float m, c, s0;
+    float2 s;
+    __device__ __forceinline__ Running() : m(-INFINITY), c(0.0f), s0(0.0f), s(both(0.0f)) {}
+    __device__ __forceinline__ void raise(float top, float k) {
+        if (top > m) {
+            const float old = c;
+            const bool first = is_far(m, k);
+            m = top;
+            c = is_far(m, k) ? 0.0f : -m * k;
+            if (!first) {
+                const float f = fast_exp2(c - old);
+                s = mul2(s, both(f));
+                s0 *= f;
             }
         }
+    }
+    __device__ __forceinline__ void add(float x, float k, float rest) {
+        raise(x, k);
+        s0 += fast_exp2(fmaf(x, rest, fmaf(x, k, c)));
     }
 };
 
-// Running maximum m and sum s of exp2((x - m) * k).  One vector at a time: its maximum decides
-// whether the sum is rescaled, rare after the first few.
-template <int N>
-__device__ __forceinline__ void take(const float (&v)[N], float k, float& m, float& s) {
-    float top = v[0];
-    #pragma unroll
-    for (int j = 1; j < N; ++j) top = fmaxf(top, v[j]);
-    if (top > m) { s *= fast_exp2((m - top) * k); m = top; }
-    if (m == -CUDART_INF_F) {                        // nothing finite yet; a NaN must not get lost
-        #pragma unroll
-        for (int j = 0; j < N; ++j) if (v[j] != v[j]) s = v[j];
-        return;
-    }
-    #pragma unroll
-    for (int j = 0; j < N; ++j) s += fast_exp2((v[j] - m) * k);
+// (m, sum of 2^(x k - m k)) of this block's share of the row, in every thread.
+struct Stats { float m, s; };
+
+__device__ __forceinline__ Stats merge(Stats a, Stats b, float k) {
+    const float top = fmaxf(a.m, b.m);
+    if (top == -INFINITY) return Stats{top, a.s + b.s};
+    return Stats{top, a.s * fast_exp2((a.m - top) * k) + b.s * fast_exp2((b.m - top) * k)};
 }
 
-__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float k) {
-    const float top = fmaxf(m, m2);
-    if (top == -CUDART_INF_F) { s += s2; return; }
-    s = s * fast_exp2((m - top) * k) + s2 * fast_exp2((m2 - top) * k);
-    m = top;
-}
-
-// (maximum, sum) of the row, in every thread.
 template <typename T>
-__device__ float2 row_stats(const Row<T>& row, float k) {
-    constexpr int N = Row<T>::N;
-    float m = -CUDART_INF_F, s = 0.0f;
-    int i = threadIdx.x;
-    for (; i + THREADS < row.full_hi; i += 2 * THREADS) {
-        if (i >= row.full_lo) {
-            Pack16<T> a, b;
-            a.load(row.base + (long long)i * N);
-            b.load(row.base + (long long)(i + THREADS) * N);
-            float v[N];
-            a.get(v);
-            take<N>(v, k, m, s);
-            b.get(v);
-            take<N>(v, k, m, s);
-        } else {
-            float v[N];
-            row.load(i, v);
-            take<N>(v, k, m, s);
-            row.load(i + THREADS, v);
-            take<N>(v, k, m, s);
-        }
+__device__ Stats row_stats(const Row<T>& row, float k, float rest, bool with_edges, Stats* part) {
+    constexpr int P = Row<T>::P;
+    Running run;
+    const float2 k2 = both(k), rest2 = both(rest);
+    auto take = [&](const uint4& q) {
+        float2 v[P];
+        Pack<T>::pairs(q, v);
+        const float2 c2 = both(run.c);
+        #pragma unroll
+        for (int j = 0; j < P; ++j) run.s = add2(run.s, exp2_2(fma2(v[j], rest2, fma2(v[j], k2, c2))));
+    };
+    int i = row.lo + (int)threadIdx.x;
+    for (; i + (BATCH - 1) * THREADS < row.hi; i += BATCH * THREADS) {
+        uint4 q[BATCH];
+        #pragma unroll
+        for (int u = 0; u < BATCH; ++u) q[u] = row.base[i + u * THREADS];
+        run.raise(Pack<T>::top(q), k);
+        #pragma unroll
+        for (int u = 0; u < BATCH; ++u) take(q[u]);
     }
-    for (; i < row.vectors; i += THREADS) {
-        float v[N];
-        row.load(i, v);
-        take<N>(v, k, m, s);
+    for (; i < row.hi; i += THREADS) {
+        const uint4 q[1] = {row.base[i]};
+        run.raise(Pack<T>::top(q), k);
+        take(q[0]);
     }
-    __shared__ float2 part[THREADS / 32];
+    if (with_edges && (int)threadIdx.x < row.edges()) run.add(gb_up(row.x[row.edge(threadIdx.x)]), k, rest);
+    Stats mine{run.m, run.s.x + run.s.y + run.s0};
+    // the sums are of 2^(x log2(e) / T + c): what c differs from the maximum's is put right once a thread
+    if (!is_far(mine.m, k)) mine.s *= fast_exp2(fmaf(-mine.m, rest, fmaf(-mine.m, k, -run.c)));
+    float top = mine.m;
     #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-        merge(m, s, m2, s2, k);
-    }
-    __syncthreads();                                 // the last row's results may still be read
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(m, s);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top != -INFINITY) mine.s *= fast_exp2((mine.m - top) * k);
+    mine.s = gb_warp_sum(mine.s);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = Stats{top, mine.s};
     __syncthreads();
-    m = part[0].x; s = part[0].y;
+    Stats all = part[0];
     #pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) merge(m, s, part[w].x, part[w].y, k);
-    return make_float2(m, s);
+    for (int w = 1; w < WARPS; ++w) all = merge(all, part[w], k);
+    return all;
 }
 
-// The gradient of a row whose log-probability has the gradient `coef`: zeros from vocab to ld.
-// `out` lies in its vectors as the row does.
+// The sum alone of a block's share, by differences, for a maximum that is far.
 template <typename T>
-__device__ void write_grad(const Row<T>& row, T* out, int ld, int target, float coef, float2 stats, float k,
-                           float inv_temperature) {
-    constexpr int N = Row<T>::N;
-    const float scale = -coef * inv_temperature / stats.y, hit = coef * inv_temperature;
-    T* base = out - row.skew;
-    const int vectors = (ld + row.skew + N - 1) / N, full_hi = (ld + row.skew) / N;
-    const int at = target + row.skew;
-    for (int i = threadIdx.x; i < vectors; i += THREADS) {
-        float v[N];
-        row.load(i, v);
+__device__ float far_sum(const Row<T>& row, float m, float k, bool with_edges, Stats* part) {
+    float s = 0.0f;
+    for (int i = row.lo + (int)threadIdx.x; i < row.hi; i += THREADS) {
+        float2 v[Row<T>::P];
+        Pack<T>::pairs(row.base[i], v);
         #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            v[j] = fast_exp2((v[j] - stats.x) * k) * scale;
-            if (!row.full(i) && i * N - row.skew + j >= row.vocab) v[j] = 0.0f;
+        for (int j = 0; j < Row<T>::P; ++j) s += fast_exp2((v[j].x - m) * k) + fast_exp2((v[j].y - m) * k);
+    }
+    if (with_edges && (int)threadIdx.x < row.edges()) s += fast_exp2((gb_up(row.x[row.edge(threadIdx.x)]) - m) * k);
+    s = gb_warp_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5].s = s;
+    __syncthreads();
+    float total = 0.0f;
+    for (int w = 0; w < WARPS; ++w) total += part[w].s;
+    return total;
+}
+
+// The gradient of this block's share of a row whose log-probability has the gradient `coef`;
+// zeros from vocab to ld.  `out` lies across its vectors as the row does.
+template <typename T>
+__device__ void write_grad(const Row<T>& row, T* out, int ld, int target, float coef, Stats stats, float k, float rest,
+                           float inv_temperature, bool with_edges) {
+    constexpr int N = Row<T>::N, P = Row<T>::P;
+    // p = 2^(x k + c) / s with c near -m k: c's rounding, and what k leaves out at m, go into s
+    const bool far = is_far(stats.m, k);
+    const float c = far ? 0.0f : -stats.m * k;
+    const float s = far ? stats.s : stats.s * fast_exp2(fmaf(stats.m, k, c)) * fast_exp2(-stats.m * rest);
+    const float scale = -coef * inv_temperature / s, hit = coef * inv_temperature;
+    const float2 k2 = both(k), c2 = both(c), scale2 = both(scale);
+    uint4* to = reinterpret_cast<uint4*>(out - row.skew);
+    const int at = (target + row.skew) / N, place = (target + row.skew) % N;
+    auto give = [&](int i, const uint4& q) {
+        float2 v[P];
+        Pack<T>::pairs(q, v);
+        #pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const float2 t = far ? make_float2((v[j].x - stats.m) * k, (v[j].y - stats.m) * k) : fma2(v[j], k2, c2);
+            v[j] = mul2(exp2_2(t), scale2);
         }
-        if (i == at / N) {
+        if (i == at) {
             #pragma unroll
-            for (int j = 0; j < N; ++j) if (j == at % N) v[j] += hit;
-        }
-        if (i >= row.full_lo && i < full_hi) Pack16<T>::store(base + (long long)i * N, v);
-        else {
-            #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int col = i * N - row.skew + j;
-                if (col >= 0 && col < ld) base[(long long)i * N + j] = gb_down<T>(v[j]);
+            for (int j = 0; j < P; ++j) {
+                if (2 * j == place) v[j].x += hit;
+                if (2 * j + 1 == place) v[j].y += hit;
             }
         }
+        to[i] = Pack<T>::back(v);
+    };
+    int i = row.lo + (int)threadIdx.x;
+    for (; i + (BATCH - 1) * THREADS < row.hi; i += BATCH * THREADS) {
+        uint4 q[BATCH];
+        #pragma unroll
+        for (int u = 0; u < BATCH; ++u) q[u] = row.base[i + u * THREADS];
+        #pragma unroll
+        for (int u = 0; u < BATCH; ++u) give(i + u * THREADS, q[u]);
     }
+    for (; i < row.hi; i += THREADS) give(i, row.base[i]);
+    if (!with_edges) return;
+    if ((int)threadIdx.x < row.edges()) {
+        const int col = row.edge(threadIdx.x);
+        const float x = gb_up(row.x[col]);
+        const float g = fast_exp2(far ? (x - stats.m) * k : fmaf(x, k, c)) * scale;
+        out[col] = gb_down<T>(col == target ? g + hit : g);
+    }
+    for (int col = row.vocab + threadIdx.x; col < ld; col += THREADS) out[col] = gb_down<T>(0.0f);
 }
 
 template <typename T>
-__device__ void write_zeros(const Row<T>& row, T* out, int ld) {
-    constexpr int N = Row<T>::N;
-    T* base = out - row.skew;
-    const int vectors = (ld + row.skew + N - 1) / N, full_hi = (ld + row.skew) / N;
-    const float zero[N] = {};
-    for (int i = threadIdx.x; i < vectors; i += THREADS) {
-        if (i >= row.full_lo && i < full_hi) Pack16<T>::store(base + (long long)i * N, zero);
-        else {
-            #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int col = i * N - row.skew + j;
-                if (col >= 0 && col < ld) base[(long long)i * N + j] = gb_down<T>(0.0f);
-            }
-        }
-    }
+__device__ void write_zeros(const Row<T>& row, T* out, int ld, bool with_edges) {
+    uint4* to = reinterpret_cast<uint4*>(out - row.skew);
+    for (int i = row.lo + (int)threadIdx.x; i < row.hi; i += THREADS) to[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (!with_edges) return;
+    if ((int)threadIdx.x < row.edges()) out[row.edge(threadIdx.x)] = gb_down<T>(0.0f);
+    for (int col = row.vocab + threadIdx.x; col < ld; col += THREADS) out[col] = gb_down<T>(0.0f);
 }
 
 // Sum over the block in 64 bits, in a fixed order, in every thread.
+template <int COUNT>
 __device__ double block_sum(double v) {
-    __shared__ double part[THREADS / 32];
+    __shared__ double part[COUNT / 32];
     v = gb_warp_sum(v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
     double total = part[0];
-    for (int w = 1; w < THREADS / 32; ++w) total += part[w];
+    for (int w = 1; w < COUNT / 32; ++w) total += part[w];
     return total;
 }
 
@@ -243,91 +371,128 @@ struct ForwardArgs {
 };
 
 enum { LOGPROBS = 0, POLICY = 1 };
+constexpr int SMALL = 1024;              // threads of the one-block kernels
 
+// The reciprocal of the denominator, which every row's coefficient needs.
+__global__ void __launch_bounds__(SMALL) policy_denominator_kernel(const ForwardArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the rows' first sweep needs nothing of this
+    double d = 0.0;
+    if (a.denominator) d = *a.denominator;
+    else {
+        for (long long r = threadIdx.x; r < a.rows.rows; r += SMALL) {
+            const long long t = a.targets[r];
+            if (t >= 0 && t < a.rows.vocab) d += a.weights ? (double)a.weights[r] : 1.0;
+        }
+        d = block_sum<SMALL>(d);
+    }
+    // where no token counts, loss and gradient are 0
+    if (threadIdx.x == 0) *a.inv_denominator = d == 0.0 ? 0.0f : (float)(1.0 / d);
+}
+
+// One row a block, or a row a cluster where there are fewer rows than the SMs can hold blocks.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(THREADS) forward_kernel(const ForwardArgs a) {
+    __shared__ Stats s_part[WARPS], s_block;
     __shared__ float s_coef;
-    float inv = 1.0f;
-    if (MODE == POLICY) {
-        double d;
-        if (a.denominator) d = *a.denominator;
-        else {                           // every block adds the weights for itself: no second launch
-            d = 0.0;
-            for (long long r = threadIdx.x; r < a.rows.rows; r += THREADS) {
-                const long long t = a.targets[r];
-                if (t >= 0 && t < a.rows.vocab) d += a.weights ? (double)a.weights[r] : 1.0;
-            }
-            d = block_sum(d);
-        }
-        inv = d == 0.0 ? 0.0f : (float)(1.0 / d);    // no token counts: loss and gradient are 0
-        if (blockIdx.x == 0 && threadIdx.x == 0) *a.inv_denominator = inv;
-    }
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const long long r = blockIdx.x / parts;
+    const bool first = rank == 0;
     const float k = LOG2E * a.inv_temperature;
-    for (long long r = blockIdx.x; r < a.rows.rows; r += gridDim.x) {
-        const long long at = a.rows.offset(r);
-        const T* x = static_cast<const T*>(a.rows.x) + at;
-        const Row<T> row(x, a.rows.vocab);
-        const long long target = a.targets[r];
-        const float weight = (MODE == POLICY && a.weights) ? a.weights[r] : 1.0f;
-        const bool counted = target >= 0 && target < a.rows.vocab && weight != 0.0f;
-        T* out = a.grad ? static_cast<T*>(a.grad) + r * a.rows.ld : nullptr;
-        if (!counted) {
-            if (threadIdx.x == 0) {
-                a.logprobs[r] = 0.0f;
-                if (a.stats) a.stats[r] = make_float2(0.0f, 1.0f);
-                if (MODE == POLICY) {
-                    a.coef[r] = 0.0f;
-                    for (int q = 0; q < 3; ++q) a.terms[q * a.rows.rows + r] = 0.0f;
-                }
-            }
-            if (out) write_zeros(row, out, a.rows.ld);
-            continue;
-        }
-        const float2 stats = row_stats(row, k);
-        if (threadIdx.x == 0) {
-            const float logprob = (gb_up(x[target]) - stats.x) * a.inv_temperature - logf(stats.y);
-            a.logprobs[r] = logprob;
-            if (a.stats) a.stats[r] = stats;
+    const float rest = fmaf(LOG2E, a.inv_temperature, -k) + LOG2E_REST * a.inv_temperature;
+    const long long at = a.rows.offset(r);
+    const T* x = static_cast<const T*>(a.rows.x) + at;
+    const Row<T> row(x, a.rows.vocab, rank, parts);
+    const long long target = a.targets[r];
+    const float weight = (MODE == POLICY && a.weights) ? a.weights[r] : 1.0f;
+    const bool counted = target >= 0 && target < a.rows.vocab && weight != 0.0f;
+    T* out = a.grad ? static_cast<T*>(a.grad) + r * a.rows.ld : nullptr;
+    if (!counted) {                      // so it is for the whole cluster
+        if (first && threadIdx.x == 0) {
+            a.logprobs[r] = 0.0f;
+            if (a.stats) a.stats[r] = make_float2(0.0f, 1.0f);
             if (MODE == POLICY) {
-                const float adv = a.advantages[r];
-                const float ratio = expf(logprob - a.old[r]);
-                const float low = 1.0f - a.clip_low, high = 1.0f + a.clip_high;
-                const bool outside = (adv > 0.0f && ratio > high) || (adv < 0.0f && ratio < low);
-                float loss = -fminf(ratio * adv, fminf(fmaxf(ratio, low), high) * adv);
-                if (ratio != ratio || adv != adv) loss = ratio * adv;        // a NaN stays one
-                float d = outside ? 0.0f : -adv * ratio;
-                float kl = 0.0f;
-                if (a.ref) {
-                    const float gap = a.ref[r] - logprob, e = expm1f(gap);
-                    kl = e - gap;
-                    loss += a.kl_coef * kl;
-                    d -= a.kl_coef * e;
-                }
+                a.coef[r] = 0.0f;
+                for (int q = 0; q < 3; ++q) a.terms[q * a.rows.rows + r] = 0.0f;
+            }
+        }
+        if (out) write_zeros(row, out, a.rows.ld, first);
+        // whoever waits for this launch may count on the one ahead of it
+        if (MODE == POLICY && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
+    Stats stats = row_stats(row, k, rest, first, s_part);
+    if (parts > 1) {
+        if (threadIdx.x == 0) s_block = stats;
+        cluster.sync();
+        stats = *cluster.map_shared_rank(&s_block, 0);
+        for (int p = 1; p < parts; ++p) stats = merge(stats, *cluster.map_shared_rank(&s_block, p), k);
+    }
+    if (is_far(stats.m, k)) {            // the same in every block of the cluster
+        stats.s = far_sum(row, stats.m, k, first, s_part);
+        if (parts > 1) {
+            cluster.sync();
+            if (threadIdx.x == 0) s_block.s = stats.s;
+            cluster.sync();
+            stats.s = 0.0f;
+            for (int p = 0; p < parts; ++p) stats.s += cluster.map_shared_rank(&s_block, p)->s;
+        }
+    }
+    if (stats.s < 1.0f) stats.s = 1.0f;  // the maximum's own term is 1: what is less is rounding
+    if (threadIdx.x == 0) {
+        const float logprob = (gb_up(x[target]) - stats.m) * a.inv_temperature - logf(stats.s);
+        if (first) {
+            a.logprobs[r] = logprob;
+            if (a.stats) a.stats[r] = make_float2(stats.m, stats.s);
+        }
+        if (MODE == POLICY) {
+            const float adv = a.advantages[r];
+            const float ratio = expf(logprob - a.old[r]);
+            const float low = 1.0f - a.clip_low, high = 1.0f + a.clip_high;
+            const bool outside = (adv > 0.0f && ratio > high) || (adv < 0.0f && ratio < low);
+            float loss = -fminf(ratio * adv, fminf(fmaxf(ratio, low), high) * adv);
+            if (ratio != ratio || adv != adv) loss = ratio * adv;        // a NaN stays one
+            float d = outside ? 0.0f : -adv * ratio;
+            float kl = 0.0f;
+            if (a.ref) {
+                const float gap = a.ref[r] - logprob, e = expm1f(gap);
+                kl = e - gap;
+                loss += a.kl_coef * kl;
+                d -= a.kl_coef * e;
+            }
+            asm volatile("griddepcontrol.wait;" ::: "memory");           // the denominator is there
+            s_coef = weight * *reinterpret_cast<volatile float*>(a.inv_denominator) * d;
+            if (first) {
                 a.terms[r] = weight * loss;
                 a.terms[a.rows.rows + r] = weight * kl;
                 a.terms[2 * a.rows.rows + r] = outside ? weight : 0.0f;
-                s_coef = weight * inv * d;
                 a.coef[r] = s_coef;
             }
         }
-        if (MODE == POLICY && out) {
-            __syncthreads();
-            const float coef = s_coef;
-            if (coef == 0.0f) write_zeros(row, out, a.rows.ld);
-            else write_grad(row, out, a.rows.ld, (int)target, coef, stats, k, a.inv_temperature);
-        }
     }
+    if (MODE == POLICY && out) {
+        __syncthreads();
+        const float coef = s_coef;
+        if (coef == 0.0f) write_zeros(row, out, a.rows.ld, first);
+        else write_grad(row, out, a.rows.ld, (int)target, coef, stats, k, rest, a.inv_temperature, first);
+    }
+    if (parts > 1) cluster.sync();       // no block leaves while another may read its result
 }
 
 // The three sums of terms times the reciprocal denominator.
-__global__ void __launch_bounds__(THREADS) policy_finish_kernel(const float* __restrict__ terms, long long rows,
-                                                                const float* inv, float* loss, float* kl,
-                                                                float* clipped) {
+struct FinishArgs {
+    const float* terms;
+    long long rows;
+    const float* inv;
+    float *loss, *kl, *clipped;
+};
+__global__ void __launch_bounds__(SMALL) policy_finish_kernel(const FinishArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int q = 0; q < 3; ++q) {
         double acc = 0.0;
-        for (long long r = threadIdx.x; r < rows; r += THREADS) acc += terms[q * rows + r];
-        acc = block_sum(acc);
-        if (threadIdx.x == 0) *(q == 0 ? loss : q == 1 ? kl : clipped) = (float)(acc * (double)*inv);
+        for (long long r = threadIdx.x; r < a.rows; r += SMALL) acc += a.terms[q * a.rows + r];
+        acc = block_sum<SMALL>(acc);
+        if (threadIdx.x == 0) *(q == 0 ? a.loss : q == 1 ? a.kl : a.clipped) = (float)(acc * (double)*a.inv);
     }
 }
 
@@ -339,20 +504,24 @@ struct GradArgs {
     const float* upstream;               // one value that multiplies every coefficient, or null
     float inv_temperature;
     void* grad;
+    int parts;                           // blocks a row
 };
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
     const float up = a.upstream ? *a.upstream : 1.0f;
     const float k = LOG2E * a.inv_temperature;
-    for (long long r = blockIdx.x; r < a.rows.rows; r += gridDim.x) {
-        const long long at = a.rows.offset(r);
-        const Row<T> row(static_cast<const T*>(a.rows.x) + at, a.rows.vocab);
-        T* out = static_cast<T*>(a.grad) + r * a.rows.ld;
-        const long long target = a.targets[r];
-        const float own = a.coef[r], coef = own * up;
-        if (target < 0 || target >= a.rows.vocab || own == 0.0f || coef == 0.0f) write_zeros(row, out, a.rows.ld);
-        else write_grad(row, out, a.rows.ld, (int)target, coef, a.stats[r], k, a.inv_temperature);
+    const float rest = fmaf(LOG2E, a.inv_temperature, -k) + LOG2E_REST * a.inv_temperature;
+    const long long r = blockIdx.x / a.parts;
+    const int part = (int)(blockIdx.x - r * a.parts);
+    const Row<T> row(static_cast<const T*>(a.rows.x) + a.rows.offset(r), a.rows.vocab, part, a.parts);
+    T* out = static_cast<T*>(a.grad) + r * a.rows.ld;
+    const long long target = a.targets[r];
+    const float own = a.coef[r], coef = own * up;
+    if (target < 0 || target >= a.rows.vocab || own == 0.0f || coef == 0.0f) write_zeros(row, out, a.rows.ld, part == 0);
+    else {
+        const float2 st = a.stats[r];
+        write_grad(row, out, a.rows.ld, (int)target, coef, Stats{st.x, st.y}, k, rest, a.inv_temperature, part == 0);
     }
 }
 
@@ -371,8 +540,9 @@ struct PreferenceArgs {
 };
 
 // One block: the log-probabilities are a few bytes a row next to the logits' hundred thousand.
-__global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArgs a) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = THREADS / 32;
+__global__ void __launch_bounds__(SMALL) preference_kernel(const PreferenceArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = SMALL / 32;
     auto begin = [&](int s) {
         long long v = a.offsets ? a.offsets[s] : s * a.length;
         return v < 0 ? 0LL : (v > a.rows ? a.rows : v);      // whatever the offsets hold, rows are in range
@@ -398,7 +568,7 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
     __syncthreads();
     const int pairs = a.sequences / 2;
     double loss = 0.0;
-    for (int p = threadIdx.x; p < pairs; p += THREADS) {
+    for (int p = threadIdx.x; p < pairs; p += SMALL) {
         auto reward = [&](int s) {
             const double ref = a.ref_double ? static_cast<const double*>(a.ref)[s] : static_cast<const float*>(a.ref)[s];
             return a.beta * (a.sums[s] - ref);
@@ -413,17 +583,61 @@ __global__ void __launch_bounds__(THREADS) preference_kernel(const PreferenceArg
         a.seq_coef[p] = (float)(d * (double)a.seq_coef[p]);
         a.seq_coef[p + pairs] = (float)(-d * (double)a.seq_coef[p + pairs]);
     }
-    loss = block_sum(loss);                          // its barriers also publish seq_coef
+    loss = block_sum<SMALL>(loss);                          // its barriers also publish seq_coef
     if (threadIdx.x == 0) *a.loss = (float)(loss / pairs);
-    for (long long r = threadIdx.x; r < begin(0); r += THREADS) a.coef[r] = 0.0f;
-    for (long long r = begin(a.sequences) + threadIdx.x; r < a.rows; r += THREADS) a.coef[r] = 0.0f;
+    for (long long r = threadIdx.x; r < begin(0); r += SMALL) a.coef[r] = 0.0f;
+    for (long long r = begin(a.sequences) + threadIdx.x; r < a.rows; r += SMALL) a.coef[r] = 0.0f;
     for (int s = warp; s < a.sequences; s += warps) {
         const float c = a.seq_coef[s];
         for (long long r = begin(s) + lane; r < begin(s + 1); r += 32) a.coef[r] = c;
     }
 }
 
-int grid_for(long long rows) { return (int)(rows < 148 * 4 ? rows : 148 * 4); }
+// Blocks that share a row: as many as keep the SMs busy (five blocks fit on each), but not less
+// than two vectors for every thread of them, and no more than a cluster may have.
+int parts_for(long long rows, int vocab, int width) {
+    const long long vectors = (long long)vocab * width / 16;
+    int parts = 1;
+    while (parts < 8 && rows * parts * 2 <= 148 * 5 && vectors >= (long long)parts * 2 * THREADS * 2) parts *= 2;
+    return parts;
+}
+
+// A launch of clusters of `parts` blocks.  `early`: it may begin before the launch ahead of it is done,
+// which it waits for where it needs it.
+template <typename K, typename A>
+int start(K kernel, long long grid, int threads, int parts, bool early, cudaStream_t stream, A args) {
+    if (grid > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    cudaLaunchAttribute attr[2] = {};
+    int n = 0;
+    if (parts > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)parts;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (early) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)grid);
+    config.blockDim = dim3(threads);
+    config.stream = stream;
+    config.attrs = attr;
+    config.numAttrs = n;
+    return (int)cudaLaunchKernelEx(&config, kernel, args);
+}
+
+template <int MODE>
+int start_forward(int dtype, const ForwardArgs& a, bool early, cudaStream_t stream) {
+    const int parts = parts_for(a.rows.rows, a.rows.vocab, dtype == GB_F32 ? 4 : 2);
+    const long long grid = a.rows.rows * parts;
+    if (dtype == GB_F32) return start(forward_kernel<float, MODE>, grid, THREADS, parts, early, stream, a);
+    if (dtype == GB_BF16) return start(forward_kernel<__nv_bfloat16, MODE>, grid, THREADS, parts, early, stream, a);
+    if (dtype == GB_F16) return start(forward_kernel<__half, MODE>, grid, THREADS, parts, early, stream, a);
+    return (int)cudaErrorInvalidValue;
+}
 
 bool bad(const Rows& r) {
     return r.rows <= 0 || r.inner <= 0 || r.vocab <= 0 || r.ld < r.vocab || r.ld > 0x7fffff00;
@@ -443,12 +657,7 @@ extern "C" int gb_token_logprobs(int dtype, const void* logits, long long batch_
     if (bad(a.rows)) return (int)cudaErrorInvalidValue;
     a.targets = targets; a.inv_temperature = 1.0f / temperature; a.logprobs = logprobs;
     a.stats = reinterpret_cast<float2*>(stats);
-    const int grid = grid_for(rows);
-    if (dtype == GB_F32) forward_kernel<float, LOGPROBS><<<grid, THREADS, 0, stream>>>(a);
-    else if (dtype == GB_BF16) forward_kernel<__nv_bfloat16, LOGPROBS><<<grid, THREADS, 0, stream>>>(a);
-    else if (dtype == GB_F16) forward_kernel<__half, LOGPROBS><<<grid, THREADS, 0, stream>>>(a);
-    else return (int)cudaErrorInvalidValue;
-    return (int)cudaGetLastError();
+    return start_forward<LOGPROBS>(dtype, a, false, stream);
 }
 
 // scratch: 3 * rows + 1 floats.  loss, kl, clipped (share): one float each.  ref, weights and denominator may be
@@ -467,15 +676,11 @@ extern "C" int gb_policy_loss(int dtype, const void* logits, long long batch_str
     a.old = old; a.advantages = advantages; a.ref = ref; a.weights = weights; a.denominator = denominator;
     a.clip_low = clip_low; a.clip_high = clip_high; a.kl_coef = kl_coef;
     a.coef = coef; a.terms = scratch; a.inv_denominator = scratch + 3 * rows; a.grad = grad;
-    const int grid = grid_for(rows);
-    if (dtype == GB_F32) forward_kernel<float, POLICY><<<grid, THREADS, 0, stream>>>(a);
-    else if (dtype == GB_BF16) forward_kernel<__nv_bfloat16, POLICY><<<grid, THREADS, 0, stream>>>(a);
-    else if (dtype == GB_F16) forward_kernel<__half, POLICY><<<grid, THREADS, 0, stream>>>(a);
-    else return (int)cudaErrorInvalidValue;
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return (int)err;
-    policy_finish_kernel<<<1, THREADS, 0, stream>>>(scratch, rows, scratch + 3 * rows, loss, kl, clipped);
-    return (int)cudaGetLastError();
+    int err = start(policy_denominator_kernel, 1, SMALL, 1, false, stream, a);
+    if (err) return err;
+    if ((err = start_forward<POLICY>(dtype, a, true, stream))) return err;
+    const FinishArgs f = {scratch, rows, scratch + 3 * rows, loss, kl, clipped};
+    return start(policy_finish_kernel, 1, SMALL, 1, true, stream, f);
 }
 
 extern "C" int gb_logprob_grad(int dtype, const void* logits, long long batch_stride, long long row_stride,
@@ -487,12 +692,12 @@ extern "C" int gb_logprob_grad(int dtype, const void* logits, long long batch_st
     if (bad(a.rows)) return (int)cudaErrorInvalidValue;
     a.targets = targets; a.stats = reinterpret_cast<const float2*>(stats); a.coef = coef; a.upstream = upstream;
     a.inv_temperature = 1.0f / temperature; a.grad = grad;
-    const int grid = grid_for(rows);
-    if (dtype == GB_F32) grad_kernel<float><<<grid, THREADS, 0, stream>>>(a);
-    else if (dtype == GB_BF16) grad_kernel<__nv_bfloat16><<<grid, THREADS, 0, stream>>>(a);
-    else if (dtype == GB_F16) grad_kernel<__half><<<grid, THREADS, 0, stream>>>(a);
-    else return (int)cudaErrorInvalidValue;
-    return (int)cudaGetLastError();
+    a.parts = parts_for(rows, vocab, dtype == GB_F32 ? 4 : 2);
+    const long long grid = rows * a.parts;
+    if (dtype == GB_F32) return start(grad_kernel<float>, grid, THREADS, 1, false, stream, a);
+    if (dtype == GB_BF16) return start(grad_kernel<__nv_bfloat16>, grid, THREADS, 1, false, stream, a);
+    if (dtype == GB_F16) return start(grad_kernel<__half>, grid, THREADS, 1, false, stream, a);
+    return (int)cudaErrorInvalidValue;
 }
 
 // sums: `sequences` doubles of scratch, seq_coef: as many floats.  The first half of the sequences
@@ -505,6 +710,5 @@ extern "C" int gb_preference_loss(const float* logprobs, const long long* target
     if (sequences < 2 || sequences % 2) return (int)cudaErrorInvalidValue;
     const PreferenceArgs a = {logprobs, targets, offsets, rows, length, sequences, vocab, average, ref, ref_double,
                               beta, smoothing, sums, seq_coef, loss, rewards, seq_logprobs, coef};
-    preference_kernel<<<1, THREADS, 0, stream>>>(a);
-    return (int)cudaGetLastError();
+    return start(preference_kernel, 1, SMALL, 1, true, stream, a);
 }
