@@ -40,6 +40,7 @@ import torch.distributed as dist
 
 import gpubridge_b200 as gb
 from gpubridge_b200.models import llama
+from gpubridge_b200.ops.grad_clip import clip_grad_norm_
 
 
 def shares_for(weights: list[float], total: int) -> list[int]:
@@ -55,6 +56,19 @@ def shares_for(weights: list[float], total: int) -> list[int]:
     for r in order[:total - sum(shares)]:
         shares[r] += 1
     return shares
+
+
+def clip(args, model, replicated=None) -> None:
+    """Clip the gradients by the norm of the whole model's: ``single`` and ``ddp`` hold them whole,
+    ``fused`` joins its shards' norms, ``fsdp2`` and ``hsdp`` hold DTensors, which torch clips."""
+    if args.clip_norm is None:
+        return
+    if args.mode == "fused":
+        replicated.clip_gradients(args.clip_norm)
+    elif args.mode in ("fsdp2", "hsdp"):
+        torch.nn.utils.clip_grad_norm_(model.parameters(), args.clip_norm)
+    else:
+        clip_grad_norm_(model.parameters(), args.clip_norm)
 
 
 def _digest(tensors) -> tuple[str, float]:
@@ -192,6 +206,7 @@ def recorded(args) -> int:
             local_loss += float(loss.detach()) if not on_gpu else loss.detach()
         if args.mode == "fused":
             replicated.average_gradients()
+        clip(args, model, replicated if args.mode == "fused" else None)
         optimizer.step()
         wait()
         times.append(max(everyone(time.perf_counter() - t0)))
@@ -238,6 +253,7 @@ def main(argv=None) -> int:
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--lr", type=float, default=3e-4)
+    ap.add_argument("--clip-norm", type=float, help="clip the gradients to this global 2-norm before the update")
     ap.add_argument("--backend", default="gpubridge", help="gpubridge or nccl (the baseline)")
     ap.add_argument("--rng", default="device", choices=("cpu", "device"),
                     help="where the random initial weights are drawn (same seed on every rank)")
@@ -308,6 +324,7 @@ def main(argv=None) -> int:
         loss.backward()
         if args.mode == "fused":
             replicated.average_gradients()
+        clip(args, model, replicated if args.mode == "fused" else None)
         optimizer.step()
         return loss.detach()
 

@@ -4,7 +4,8 @@ Architecture of the reference's ``train_bench.py`` model (scripts/gpu/train_benc
 pre-LayerNorm blocks of causal self-attention and a 4x GELU(tanh) MLP, learned positions,
 tied input/output embedding.  ``gpt2-small``: 12 layers, 12 heads, width 768, vocabulary
 50257, context 1024 (124 M parameters).  Weights are initialised N(0, 0.02), biases zero,
-LayerNorm to identity.
+LayerNorm to identity.  ``GPUBRIDGE_FUSED_JOIN=1`` adds attention's output to the stream and takes
+the LayerNorm that follows in one kernel (``ops/residual_norm.py``).
 """
 from __future__ import annotations
 
@@ -15,7 +16,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from gpubridge_b200.models.attention import causal_attention
+from gpubridge_b200.models.finetune import FineTuned, fused_join
 from gpubridge_b200.ops.layernorm import FusedLayerNorm
+from gpubridge_b200.ops.residual_norm import residual_norm
 
 
 @dataclass(frozen=True)
@@ -47,11 +50,15 @@ class Block(nn.Module):
         qkv = self.qkv(self.ln1(x)).view(b, t, 3, self.heads, w // self.heads)
         q, k, v = (z.transpose(1, 2) for z in qkv.unbind(2))
         y = causal_attention(q, k, v)
-        x = x + self.proj(y.transpose(1, 2).reshape(b, t, w))
+        y = self.proj(y.transpose(1, 2).reshape(b, t, w))
+        if fused_join():
+            x, h = residual_norm(x, y, self.ln2.weight, self.ln2.bias, eps=self.ln2.eps, kind="layer")
+            return x + self.out(F.gelu(self.fc(h), approximate="tanh"))
+        x = x + y
         return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
 
 
-class GPT(nn.Module):
+class GPT(FineTuned, nn.Module):
     def __init__(self, c: GPTConfig) -> None:
         super().__init__()
         self.config = c
@@ -82,7 +89,11 @@ class GPT(nn.Module):
         return self.ln(x)
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
-        return self.head(self.hidden(idx))[..., :self.config.vocab]
+        return self.logits(idx)[..., :self.config.vocab]
+
+    def logits(self, idx: torch.Tensor) -> torch.Tensor:
+        """Logits over the padded vocabulary (columns at or past ``config.vocab`` do not count)."""
+        return self.head(self.hidden(idx))
 
     def loss(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         from gpubridge_b200.ops.xent import fused_cross_entropy

@@ -5,6 +5,11 @@ The FSDP2 / HSDP benchmark models.  Named shapes: the reference's ``llama-tiny/1
 d_model 2048, 16 heads, FFN 5632, vocabulary 32000) and ``llama3-8b`` (32 layers, d_model 4096,
 32 query / 8 KV heads, FFN 14336, vocabulary 128256).  Weights are N(0, 0.02) from a CPU
 generator with a fixed seed, so every rank (and a single-process oracle) builds the same model.
+
+A configuration may ask for a norm behind each block as well as before it (``post_norm``), a
+learned gate on each channel of a block's output (``layer_gate``) and a scale on what it adds to the
+stream (``residual_scale``): such blocks join the stream through the fused kernel
+(``ops/residual_norm.py``).  ``GPUBRIDGE_FUSED_JOIN=1`` uses it for plain blocks too.
 """
 from __future__ import annotations
 
@@ -15,6 +20,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from gpubridge_b200.models.attention import causal_attention
+from gpubridge_b200.models.finetune import FineTuned, fused_join
+from gpubridge_b200.ops.residual_norm import residual_norm
 
 
 @dataclass(frozen=True)
@@ -28,15 +35,22 @@ class LlamaConfig:
     context: int = 2048
     rope_base: float = 10000.0
     eps: float = 1e-5
+    post_norm: bool = False
+    layer_gate: bool = False
+    residual_scale: float = 1.0
 
 
 CONFIGS = {
     "llama-tiny": LlamaConfig(2, 64, 4, 2, 176, 256, 64),
+    "llama-tiny-sandwich": LlamaConfig(2, 64, 4, 2, 176, 256, 64, post_norm=True, layer_gate=True,
+                                       residual_scale=0.5),
     "llama-mini": LlamaConfig(4, 64, 4, 2, 176, 256, 64),          # four blocks: pipelines of up to four stages on CPU
     "llama-125m": LlamaConfig(12, 768, 12, 12, 2048, 32000, 2048),
     "llama-350m": LlamaConfig(24, 1024, 16, 16, 2816, 32000, 2048),
     "llama-1b": LlamaConfig(16, 2048, 32, 8, 8192, 32000, 2048),
     "llama-1.3b": LlamaConfig(24, 2048, 16, 16, 5632, 32000, 2048),
+    "llama-1.3b-sandwich": LlamaConfig(24, 2048, 16, 16, 5632, 32000, 2048, post_norm=True, layer_gate=True,
+                                       residual_scale=0.5),
     "llama3-8b": LlamaConfig(32, 4096, 32, 8, 14336, 128256, 4096, rope_base=500000.0),
 }
 
@@ -77,6 +91,11 @@ class Block(nn.Module):
         self.gate = nn.Linear(c.width, c.ffn, bias=False)
         self.up = nn.Linear(c.width, c.ffn, bias=False)
         self.down = nn.Linear(c.ffn, c.width, bias=False)
+        self.scale, self.eps = c.residual_scale, c.eps
+        self.special = c.post_norm or c.layer_gate or c.residual_scale != 1.0
+        for name, wanted in (("attn_post", c.post_norm), ("ffn_post", c.post_norm), ("attn_gate", c.layer_gate),
+                             ("ffn_gate", c.layer_gate)):
+            setattr(self, name, nn.Parameter(torch.ones(c.width)) if wanted else None)
 
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
         b, t, _ = x.shape
@@ -86,12 +105,19 @@ class Block(nn.Module):
         v = self.wv(h).view(b, t, self.kv_heads, self.head_dim).transpose(1, 2)
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         y = causal_attention(q, k, v, enable_gqa=self.kv_heads != self.heads)
-        x = x + self.wo(y.transpose(1, 2).reshape(b, t, -1))
+        y = self.wo(y.transpose(1, 2).reshape(b, t, -1))
+        if self.special or fused_join():
+            x, h = residual_norm(x, y, self.ffn_norm.weight, post_weight=self.attn_post, gate=self.attn_gate,
+                                 scale=self.scale, eps=self.eps)
+            y = self.down(F.silu(self.gate(h)) * self.up(h))
+            return residual_norm(x, y, post_weight=self.ffn_post, gate=self.ffn_gate, scale=self.scale,
+                                 eps=self.eps).stream
+        x = x + y
         h = self.ffn_norm(x)
         return x + self.down(F.silu(self.gate(h)) * self.up(h))
 
 
-class Llama(nn.Module):
+class Llama(FineTuned, nn.Module):
     def __init__(self, c: LlamaConfig) -> None:
         super().__init__()
         self.config = c
@@ -108,6 +134,9 @@ class Llama(nn.Module):
         for block in self.blocks:
             x = block(x, cos, sin)
         return self.head(self.norm(x))
+
+    def logits(self, idx: torch.Tensor) -> torch.Tensor:
+        return self(idx)
 
     def loss(self, idx: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         from gpubridge_b200.ops.xent import fused_cross_entropy
