@@ -182,15 +182,32 @@ struct Lane {
         if (E & 1) v[P - 1].y = 0.0f;
     }
     // a parameter's values in this thread's columns; `otherwise` where there is no such parameter
+    template <bool WIDE = false>
     __device__ void param(const void* p, int code, float otherwise, float2 (&v)[P]) const {
         fill(otherwise, v);
         if (!p) return;
-        if (code == GB_F32) read(static_cast<const float*>(p), v);
-        else if (code == GB_BF16) read(static_cast<const __nv_bfloat16*>(p), v);
-        else read(static_cast<const __half*>(p), v);
+        if (code == GB_F32) read<WIDE>(static_cast<const float*>(p), v);
+        else if (code == GB_BF16) read<WIDE>(static_cast<const __nv_bfloat16*>(p), v);
+        else read<WIDE>(static_cast<const __half*>(p), v);
     }
-    template <typename T>
+    template <bool WIDE, typename T>
     __device__ void read(const T* p, float2 (&v)[P]) const {
+        if constexpr (VEC == 8 && WIDE) {
+            if (reinterpret_cast<uintptr_t>(p) % (8 * sizeof(T)) == 0) {
+                Raw8<T> raw[NV];
+                #pragma unroll
+                for (int k = 0; k < NV; ++k) if (ok[k]) raw[k].load(p + col[k]);
+                #pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    if (!ok[k]) continue;
+                    float f[8];
+                    raw[k].get(f);
+                    #pragma unroll
+                    for (int j = 0; j < 8; ++j) at(v, k * 8 + j) = f[j];
+                }
+                return;
+            }
+        }
         #pragma unroll
         for (int e = 0; e < E; ++e) if (ok[e / VEC]) at(v, e) = gb_up(p[col[e / VEC] + e % VEC]);
     }
@@ -413,7 +430,9 @@ __device__ float2 row_stats(const Lane<VEC, NV>& lane, float2 (&v)[Lane<VEC, NV>
 extern __shared__ __align__(16) char join_shared[];
 
 // FULL: layer norms, or any bias; otherwise rms norms without.
-template <typename TS, typename TU, typename TY, int VEC, int NV, bool FULL>
+// OWN: the update has a norm or a gate of its own.
+template <int VEC, int NV, bool FULL, bool OWN> constexpr bool FORWARD_SHARED = FULL && OWN && VEC * NV > 8 && NV < 16;
+template <typename TS, typename TU, typename TY, int VEC, int NV, bool FULL, bool OWN>
 __global__ void __launch_bounds__(NV == 3 ? 384 : MAX_THREADS) join_fwd_kernel(const JoinArgs a) {
     __shared__ __align__(16) float buffer[REDUCER_FLOATS];
     using L = Lane<VEC, NV>;
@@ -421,7 +440,7 @@ __global__ void __launch_bounds__(NV == 3 ? 384 : MAX_THREADS) join_fwd_kernel(c
     if (team_of_grid() >= a.owners) return;          // a team's barriers are its own
     const L lane(a.d);
     const long long lo = first_row(team_of_grid(), a.rows, a.owners), hi = first_row(team_of_grid() + 1LL, a.rows, a.owners);
-    constexpr bool SHARED = FULL && VEC * NV > 8 && NV < 16;
+    constexpr bool SHARED = FORWARD_SHARED<VEC, NV, FULL, OWN>;
     using H = Held<VEC, NV, SHARED>;
     const uint32_t per_slot = (Feed<TS, VEC, NV>::BYTES + Feed<TU, VEC, NV>::BYTES) * blockDim.x;
     const uint32_t held_bytes = H::BYTES * blockDim.x;
@@ -447,20 +466,18 @@ __global__ void __launch_bounds__(NV == 3 ? 384 : MAX_THREADS) join_fwd_kernel(c
     H weight, bias, post_weight, post_bias;
     auto hold = [&](H& held, const void* p, float otherwise, int i) {
         float2 v[P];
-        lane.param(p, a.param_code, otherwise, v);
+        lane.template param<true>(p, a.param_code, otherwise, v);
         held.set(v, held_at + i * held_bytes);
     };
     hold(weight, a.weight, 1.0f, 0);
-    hold(post_weight, a.post_weight, 1.0f, 1);
-    if (FULL) {
-        hold(bias, a.bias, 0.0f, 2);
-        hold(post_bias, a.post_bias, 0.0f, 3);
-    }
+    if (FULL) hold(bias, a.bias, 0.0f, 1);
+    if (OWN) hold(post_weight, a.post_weight, 1.0f, 2);
+    if (OWN && FULL) hold(post_bias, a.post_bias, 0.0f, 3);
     Gate<VEC, NV, SHARED> gate(a, lo, gate_at);
     uint32_t slot = 0;
     const uint32_t last_slot = (a.slots - 1) * per_slot;
     for (long long row = lo; row < hi; ++row) {
-        if (row >= gate.end) gate.move(a, lane, row);
+        if (OWN && row >= gate.end) gate.move(a, lane, row);
         feed_wait(a.slots - 1);
         float2 u[P], r[P];
         from_update.get(lane, slot, u);
@@ -470,7 +487,7 @@ __global__ void __launch_bounds__(NV == 3 ? 384 : MAX_THREADS) join_fwd_kernel(c
         feed_commit();
         slot = slot == last_slot ? 0 : slot + per_slot;
         float2 post = make_float2(0.0f, 1.0f), next = make_float2(0.0f, 1.0f);
-        if (a.post_weight) {
+        if (OWN && a.post_weight) {
             post = row_stats<FULL>(lane, u, a.layer, inv_d, a.eps, reduce);
             float2 pw[P], pb[P];
             post_weight.get(pw);
@@ -483,7 +500,8 @@ __global__ void __launch_bounds__(NV == 3 ? 384 : MAX_THREADS) join_fwd_kernel(c
         }
         {
             float2 g[P];
-            gate.held.get(g);
+            if (OWN) gate.held.get(g);
+            else lane.fill(a.scale, g);
             #pragma unroll
             for (int e = 0; e < P; ++e)          // the norm that follows is that of the stream as it is stored
                 r[e] = rounded<TS>(fma2(g[e], u[e], r[e]));
@@ -583,7 +601,7 @@ __global__ void __launch_bounds__(MOST) join_bwd_kernel(const JoinArgs a) {
     H weight, post_weight, post_bias;
     auto hold = [&](H& held, const void* p, float otherwise) {
         float2 v[P];
-        lane.param(p, a.param_code, otherwise, v);
+        lane.template param<true>(p, a.param_code, otherwise, v);
         held.set(v, held_at);
         held_at += held_bytes;
     };
@@ -724,51 +742,59 @@ struct SumArgs {
     int d, sums, param_code, gate_code;
 };
 
-// Column sums of the partial results.  A block takes eight columns, one 32-byte sector of a partial
-// row, and SLICES threads share a column, four partial results under way in each: there are more
-// blocks than SMs even for one parameter of 1200 columns.
-constexpr int SLICES = 64;
-__global__ void __launch_bounds__(8 * SLICES) join_sum_kernel(const SumArgs a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");           // the partial results are there
-    const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
-    const int col = blockIdx.y * 8 + x;
+// Column sums of the partial results: a block takes 32 columns, W at a load, and its threads share
+// their partial rows, of which there is one an SM.
+template <int W>
+__global__ void __launch_bounds__(256) join_sum_kernel(const SumArgs a) {
+    constexpr int ACROSS = 32 / W, SLICES = 256 / ACROSS;
+    const int x = threadIdx.x % ACROSS, y = threadIdx.x / ACROSS;
+    const int col = blockIdx.y * 32 + x * W;
     const long long which = blockIdx.x;
     const float* base;
-    long long lo = 0, hi = a.blocks;
+    int lo = 0, hi = a.blocks;
     size_t stride;
     if (which < a.sums) {
         base = a.part + which * a.d;
         stride = (size_t)a.sums * a.d;
     } else {
         const long long g = which - a.sums;
-        lo = owner_of(g * a.group_rows, a.rows, a.owners);
-        hi = owner_of((g + 1) * a.group_rows - 1, a.rows, a.owners) + 1;
+        if (a.groups == 1) hi = a.owners;
+        else {
+            lo = (int)owner_of(g * a.group_rows, a.rows, a.owners);
+            hi = (int)owner_of((g + 1) * a.group_rows - 1, a.rows, a.owners) + 1;
+        }
         base = a.gate_part + g * a.d;
         stride = a.d;
     }
-    float acc = 0.0f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");           // the partial results are there
+    float acc[W];
+    #pragma unroll
+    for (int j = 0; j < W; ++j) acc[j] = 0.0f;
     if (col < a.d) {
-        long long c = lo + y;
-        for (; c + 3 * SLICES < hi; c += 4 * SLICES) {
-            float v[4];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = base[(c + i * SLICES) * stride + col];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) acc += v[i];
+        const float* from = base + (size_t)(lo + y) * stride + col;
+        #pragma unroll 4
+        for (int c = lo + y; c < hi; c += SLICES, from += SLICES * stride) {
+            if constexpr (W == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(from);
+                acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
+            } else acc[0] += *from;
         }
-        for (; c < hi; c += SLICES) acc += base[c * stride + col];
     }
-    acc += __shfl_xor_sync(0xffffffffu, acc, 8);                 // four slices a warp
-    acc += __shfl_xor_sync(0xffffffffu, acc, 16);
-    __shared__ float slice[SLICES / 4][8];
-    if ((threadIdx.x & 31) < 8) slice[threadIdx.x >> 5][x] = acc;
+    __shared__ float slice[SLICES][33];
+    #pragma unroll
+    for (int j = 0; j < W; ++j) slice[y][x * W + j] = acc[j];
     __syncthreads();
-    if (threadIdx.x < 8 && col < a.d) {
-        float total = slice[0][x];
-        #pragma unroll
-        for (int s = 1; s < SLICES / 4; ++s) total += slice[s][x];
-        if (which < a.sums) gb_write(a.out[which], a.param_code, col, total);
-        else gb_write(a.gate_out, a.gate_code, (size_t)(which - a.sums) * a.d + col, total);
+    // eight threads a column, each an eighth of its slices
+    const int mine = threadIdx.x / 8, part = threadIdx.x % 8;
+    float total = 0.0f;
+    #pragma unroll
+    for (int s = part; s < SLICES; s += 8) total += slice[s][mine];
+    #pragma unroll
+    for (int o = 4; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int out = blockIdx.y * 32 + mine;
+    if (part == 0 && out < a.d) {
+        if (which < a.sums) gb_write(a.out[which], a.param_code, out, total);
+        else gb_write(a.gate_out, a.gate_code, (size_t)(which - a.sums) * a.d + out, total);
     }
 }
 
@@ -846,8 +872,10 @@ template <typename TS, typename TU, typename TY, int VEC, int NV, int MOST, bool
 int launch_form(bool forward, const Shape& shape, const JoinArgs& a, cudaStream_t s) {
     constexpr int S = Feed<TS, VEC, NV>::BYTES, U = Feed<TU, VEC, NV>::BYTES, Y = Feed<TY, VEC, NV>::BYTES;
     if (forward) {
-        constexpr int H = Held<VEC, NV, (FULL && VEC * NV > 8 && NV < 16)>::BYTES;
-        return start(join_fwd_kernel<TS, TU, TY, VEC, NV, FULL>, shape, S + U, 4 * H, H, 0, a, s);
+        constexpr int H = Held<VEC, NV, FORWARD_SHARED<VEC, NV, FULL, true>>::BYTES;
+        if (a.post_weight || a.gate)
+            return start(join_fwd_kernel<TS, TU, TY, VEC, NV, FULL, true>, shape, S + U, 4 * H, H, 0, a, s);
+        return start(join_fwd_kernel<TS, TU, TY, VEC, NV, FULL, false>, shape, S + U, 0, 0, 0, a, s);
     }
     if constexpr (VEC * NV == 1) return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, false>(shape, a, s);
     else {
@@ -957,10 +985,10 @@ extern "C" int gb_residual_norm_bwd(int s, int u, int y, int vec, const void* d_
     overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     overlap.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)what, (d + 7) / 8);
-    config.blockDim = dim3(8 * SLICES);
+    config.gridDim = dim3((unsigned)what, (d + 31) / 32);
+    config.blockDim = dim3(256);
     config.stream = cuda_stream;
     config.attrs = &overlap;
     config.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&config, join_sum_kernel, q);
+    return (int)cudaLaunchKernelEx(&config, d % 4 ? join_sum_kernel<1> : join_sum_kernel<4>, q);
 }
