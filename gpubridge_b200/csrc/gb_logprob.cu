@@ -476,8 +476,9 @@ __global__ void __launch_bounds__(THREADS, 5) forward_kernel(const ForwardArgs a
             const float ratio = expf(logprob - old);
             const float low = 1.0f - a.clip_low, high = 1.0f + a.clip_high;
             const bool outside = (adv > 0.0f && ratio > high) || (adv < 0.0f && ratio < low);
-            float loss = -fminf(ratio * adv, fminf(fmaxf(ratio, low), high) * adv);
-            if (ratio != ratio || adv != adv) loss = ratio * adv;        // a NaN stays one
+            const float raw = ratio * adv;
+            float loss = -fminf(raw, fminf(fmaxf(ratio, low), high) * adv);
+            if (raw != raw) loss = raw;                                  // a NaN stays one
             float d = outside ? 0.0f : -adv * ratio;
             float kl = 0.0f;
             if (a.ref) {

@@ -803,7 +803,8 @@ constexpr int MAX_WIDTH = 8192;
 // How rows of d values in vectors of vec are dealt out: threads of a team, teams of a block, rounds
 // of vectors a thread.  Eight columns a thread up to 256, then 16 or 24: what a row costs beside
 // its values (addresses, the reduction) is shared by more of them.  Up to 768 columns a row is a
-// warp's, without a barrier.  Single values: up to four rounds of 256 threads, then sixteen of 512.
+// warp's, without a barrier.  Single values: four a thread, and up to sixteen where that is more
+// threads than a block may have.
 // A block has as many teams as its registers allow (128 a thread forward, 168 backward up to 4096
 // columns), fewer where there are not rows enough for every SM.
 struct Shape { int threads, teams, rounds; };
@@ -815,7 +816,7 @@ Shape shape_of(long long rows, int d, int vec, bool forward) {
         s.threads = vectors <= 96 ? 32 : ((vectors + 1) / 2 + 31) / 32 * 32;
     } else {
         const int most = vectors > 1024 ? MAX_THREADS : 256;
-        s.threads = (vectors + 31) / 32 * 32;
+        s.threads = ((vectors + 3) / 4 + 31) / 32 * 32;
         if (s.threads > most) s.threads = most;
         s.rounds = (vectors + s.threads - 1) / s.threads;
     }
@@ -877,16 +878,13 @@ int launch_form(bool forward, const Shape& shape, const JoinArgs& a, cudaStream_
             return start(join_fwd_kernel<TS, TU, TY, VEC, NV, FULL, true>, shape, S + U, 4 * H, H, 0, a, s);
         return start(join_fwd_kernel<TS, TU, TY, VEC, NV, FULL, false>, shape, S + U, 0, 0, 0, a, s);
     }
-    if constexpr (VEC * NV == 1) return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, false>(shape, a, s);
-    else {
-        // the widest rows with four parameters leave no room for a slot: registers hold them
-        if constexpr (MOST == 512 && FULL) {
-            constexpr int H = Held<VEC, NV, true>::BYTES;
-            if ((4 * H + 2 * S + Y + U) * shape.threads > MAX_SHARED)
-                return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, false>(shape, a, s);
-        }
-        return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, true>(shape, a, s);
+    // the widest rows of fp32 with four parameters leave no room for a slot: registers hold those
+    if constexpr (MOST == 512 && FULL && sizeof(TU) == 4) {
+        constexpr int H = Held<VEC, NV, true>::BYTES;
+        if ((4 * H + 2 * S + Y + U) * shape.threads > MAX_SHARED)
+            return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, false>(shape, a, s);
     }
+    return launch_backward<TS, TU, TY, VEC, NV, MOST, FULL, true>(shape, a, s);
 }
 
 template <typename TS, typename TU, typename TY, int VEC, int NV, int MOST>
@@ -904,8 +902,7 @@ int launch(bool forward, int vec, const JoinArgs& a, cudaStream_t s) {
         if (shape.threads * shape.teams <= 384) return launch_shaped<TS, TU, TY, 8, 2, 384>(forward, shape, a, s);
         return launch_shaped<TS, TU, TY, 8, 2, 512>(forward, shape, a, s);
     }
-    if (shape.rounds <= 1) return launch_shaped<TS, TU, TY, 1, 1, 384>(forward, shape, a, s);
-    if (shape.rounds <= 4) return launch_shaped<TS, TU, TY, 1, 4, 384>(forward, shape, a, s);
+    if (shape.rounds <= 4 && (forward || shape.threads <= 384)) return launch_shaped<TS, TU, TY, 1, 4, 384>(forward, shape, a, s);
     return launch_shaped<TS, TU, TY, 1, 16, 512>(forward, shape, a, s);
 }
 

@@ -240,6 +240,9 @@ std::optional<std::tuple<Tensor, Maybe>> residual_norm(const Tensor& residual, T
     if (code_of(residual.scalar_type()) < 0 || code_of(out) < 0) return std::nullopt;
     if (residual.scalar_type() != at::kFloat && out != residual.scalar_type()) return std::nullopt;
     if (update.device() != residual.device()) return std::nullopt;
+    // a stream and an update in fp32 are joined and normed in fp32; only the result is then rounded
+    const at::ScalarType asked = out;
+    if (residual.scalar_type() == at::kFloat && update.scalar_type() == at::kFloat) out = at::kFloat;
     if (update.scalar_type() != out) update = update.to(out);
     Tensor params[4] = {of(weight_), of(bias_), of(post_weight_), of(post_bias_)};
     if ((params[1].defined() && !params[0].defined()) || (params[3].defined() && !params[2].defined())) return std::nullopt;
@@ -267,12 +270,12 @@ std::optional<std::tuple<Tensor, Maybe>> residual_norm(const Tensor& residual, T
         at::NoGradGuard no_grad;
         auto [stream, normed, stats] = join_forward(
             Join{residual, update, params[0], params[1], params[2], params[3], gate, scale, eps, layer, out}, false);
-        return std::make_tuple(stream, normed.defined() ? Maybe(normed) : Maybe());
+        return std::make_tuple(stream, normed.defined() ? Maybe(normed.to(asked)) : Maybe());
     }
     auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
     auto got = ResidualNorm::apply(residual, update, maybe(params[0]), maybe(params[1]), maybe(params[2]), maybe(params[3]),
                                    maybe(gate), scale, eps, layer, static_cast<int64_t>(out));
-    return std::make_tuple(got[0], got.size() > 1 ? Maybe(got[1]) : Maybe());
+    return std::make_tuple(got[0], got.size() > 1 ? Maybe(got[1].to(asked)) : Maybe());
 }
 
 // -- log-probabilities -------------------------------------------------------------------------------

@@ -116,9 +116,9 @@ def grad_norm(tensors: Iterable[torch.Tensor] | torch.Tensor, norm_type: float =
 def _refuse_overlap(tensors) -> None:
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors
                    if t.numel() and _dense(t))
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
-            raise ValueError("two of the gradients share memory: it would be scaled twice")
+    gappy = [t.data_ptr() for t in tensors if t.numel() and not _dense(t)]     # these may lie between one another
+    if any(start < end for (_, end), (start, _) in zip(spans, spans[1:])) or len(set(gappy)) < len(gappy):
+        raise ValueError("two of the gradients share memory: it would be scaled twice")
 
 
 def _scale_(tensors, result: torch.Tensor) -> None:

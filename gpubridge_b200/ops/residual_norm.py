@@ -112,7 +112,8 @@ def residual_norm(residual: torch.Tensor, update: torch.Tensor, weight: torch.Te
 
     Differentiable in every tensor, once.  Types on the GPU: stream, update and ``normed`` are all
     float32, all bfloat16 or all float16, or a float32 stream with update and ``normed`` in one of
-    the others; an update of another type is converted to ``normed``'s.
+    the others.  A float32 update of a float32 stream keeps its precision, whatever ``normed``'s type;
+    any other update is converted to ``normed``'s.
     """
     if residual.is_cuda:
         got = _build_ops.load().residual_norm(residual, update, weight, bias, post_weight, post_bias, gate, scale, eps,

@@ -146,6 +146,9 @@ def test_refusals():
         clip_grad_norm_(_with_grads([t[:40], t[20:]]), 1.0)
     with pytest.raises(ValueError, match="share memory"):
         clip_grad_norm_(_with_grads([t, t]), 1.0)
+    square = _tensors(torch.float32, [64])[0].view(8, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_(_with_grads([square[:, 2:], square[:, 2:]]), 1.0)
 
 
 def test_two_streams_and_a_replayed_graph():

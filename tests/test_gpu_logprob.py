@@ -194,7 +194,7 @@ def test_policy_loss(dtype, unit_grad, weights, ref):
     loss, kl, clipped, coef, p, counted, slope, lp = _policy_wide(c, kl_coef, 0.1, 0.3)
     off = LOGPROB_TOL * slope.sum() + 8 * H
     assert ((out.logprobs - lp).abs() <= LOGPROB_TOL).all()
-    assert abs(float(out.loss) - float(loss)) <= float(off)
+    assert abs(float(out.loss.detach()) - float(loss)) <= float(off)
     assert abs(float(out.kl) - float(kl)) <= LOGPROB_TOL * 2
     assert abs(float(out.clipped) - float(clipped)) <= 4 * H
     if unit_grad:
@@ -235,6 +235,19 @@ def test_policy_loss_without_a_counting_token():
             assert float(out.loss) == 0.0 and float(out.kl) == 0.0 and float(out.clipped) == 0.0
             out.loss.backward()
             assert (logits.grad == 0).all()
+
+
+def test_policy_loss_keeps_a_nan():
+    """exp overflows against an old log-probability far below: 0 times inf is a NaN, in loss and gradient."""
+    from gpubridge_b200.ops.logprob import policy_loss
+    logits = torch.randn(2, 50, device=DEV).requires_grad_(True)
+    targets = torch.tensor([3, 4], device=DEV)
+    old = torch.tensor([-200.0, -3.0], device=DEV)
+    for unit_grad in (False, True):
+        out = policy_loss(logits, targets, old, torch.tensor([0.0, 1.0], device=DEV), unit_grad=unit_grad)
+        assert out.loss.isnan()
+        grad, = torch.autograd.grad(out.loss, logits)
+        assert grad[0].isnan().all() and torch.isfinite(grad[1]).all()
 
 
 def _preference_wide(lp, counted, bounds, ref, beta, smoothing, average):

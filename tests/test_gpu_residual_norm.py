@@ -145,7 +145,7 @@ TYPES = {"fp32": (F32, F32, F32), "autocast": (F32, BF16, F32), "autocast-fp16":
 
 @pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("kind", ["rms", "layer"])
-@pytest.mark.parametrize("width", [8, 100, 768, 1001, 2048])
+@pytest.mark.parametrize("width", [8, 100, 768, 1001, 1500, 2047, 2048])
 def test_types_and_widths(types, kind, width):
     stream, low, params = TYPES[types]
     Case((3, 37, width), kind, stream, low, params, gate="sequence", seed=width).run().check()
@@ -246,6 +246,15 @@ def test_autocast_gives_the_type_of_the_next_product():
     with torch.autocast("cuda", dtype=torch.bfloat16):
         stream, normed = residual_norm(r, u, w)
     assert stream.dtype == torch.float32 and normed.dtype == torch.bfloat16
+    # nothing was rounded before the norm's result: stream and update in fp32 are joined in fp32
+    assert torch.equal(stream, r + u)
+    full = residual_norm(r, u, w)
+    assert torch.equal(full.stream, stream) and torch.equal(full.normed.bfloat16(), normed)
+    r.requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = residual_norm(r, u, w)
+    grad, = torch.autograd.grad(out.normed.float().sum(), r)
+    assert grad.dtype == torch.float32 and torch.isfinite(grad).all()
 
 
 def test_differences():
