@@ -41,16 +41,26 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int BATCH = 4;                             // vectors of 16 bytes that a thread has under way
-// log2(e) in two parts: the rounding of one alone would shift every log-probability the same way
-// (by 1e-8 of the logits' spread, which a sum over a thousand tokens shows)
-constexpr float LOG2E = 1.4426950408889634f, LOG2E_REST = 1.9259629911266175e-8f;
-
 // 2^x by the special-function unit (2 ulp; below 2^-126 it gives 0, which no sum here resolves).
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// 2^d for a whole d, exactly: 1 above 0, 0 below -126.  1.5 * 2^23 + d has d in its last bits.
+__device__ __forceinline__ float whole_exp2(float d) {
+    return d < -126.0f ? 0.0f : __int_as_float((__float_as_int(fminf(d, 0.0f) + 12582912.0f) << 23) + 0x3f800000);
+}
+
+// The unit's powers are low by 5.0e-8 of themselves on average (4 M values in [-20, -1] on a B200;
+// their spread is 5e-8 too, but that averages out).  A sum over a thousand tokens shows it, so the
+// logarithm of a row's sum is put right by it.
+constexpr double EXP2_LOW = 5.0e-8;
+
+// log2(e) / T in two parts: the rounding of one alone would shift every log-probability the same
+// way (by 1e-8 of the logits' spread, which a sum over a thousand tokens shows as well).
+struct Base { float k, rest; double inv_temperature; };
 
 // Two values in one instruction (sm_100a's packed fp32); each rounds as the single one does.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -194,9 +204,12 @@ struct Row {
 // Where x k leaves fp32: a row whose maximum is the type's lowest value (all of it masked), or inf.
 __device__ __forceinline__ bool is_far(float m, float k) { return !(fabsf(m) * k < 1e38f); }
 
-// Running maximum m and sum s of 2^(x k + c) with c near -m k: c is held instead of m k, so what
-// its rounding is does not matter.  The maximum of a batch decides whether the sum is rescaled,
-// which is rare after the first few.  While the maximum is far, nothing is summed that counts.
+// A row's terms are 2^(x k + c) with c the whole number next to -m k, m the row's maximum: sums of
+// different c are joined by powers of two, without a rounding.
+__device__ __forceinline__ float offset_for(float m, float k) { return is_far(m, k) ? 0.0f : -rintf(m * k); }
+
+// Running maximum and sum.  The maximum of a batch decides whether the sum is rescaled, which is
+// rare after the first few.  While the maximum is far, nothing is summed that counts.
 struct Running {
     float m, c, s0;
     float2 s;
@@ -206,41 +219,52 @@ struct Running {
             const float old = c;
             const bool first = is_far(m, k);
             m = top;
-            c = is_far(m, k) ? 0.0f : -m * k;
+            c = offset_for(m, k);
             if (!first) {
-                const float f = fast_exp2(c - old);
+                const float f = whole_exp2(c - old);
                 s = mul2(s, both(f));
                 s0 *= f;
             }
         }
     }
-    __device__ __forceinline__ void add(float x, float k, float rest) {
-        raise(x, k);
-        s0 += fast_exp2(fmaf(x, rest, fmaf(x, k, c)));
+    __device__ __forceinline__ void add(float x, const Base& b) {
+        raise(x, b.k);
+        s0 += fast_exp2(fmaf(x, b.rest, fmaf(x, b.k, c)));
     }
 };
 
-// (m, sum of 2^(x k - m k)) of this block's share of the row, in every thread.
-struct Stats { float m, s; };
+// Maximum, whole number and sum of a part's terms.  A far part has no terms (its sum is 0, or a NaN).
+struct Stats { float m, c, s; };
 
-__device__ __forceinline__ Stats merge(Stats a, Stats b, float k) {
-    const float top = fmaxf(a.m, b.m);
-    if (top == -INFINITY) return Stats{top, a.s + b.s};
-    return Stats{top, a.s * fast_exp2((a.m - top) * k) + b.s * fast_exp2((b.m - top) * k)};
+template <typename F>
+__device__ __forceinline__ Stats join(int parts, float k, F part) {
+    float m = part(0).m;
+    for (int p = 1; p < parts; ++p) m = fmaxf(m, part(p).m);
+    Stats all{m, offset_for(m, k), 0.0f};
+    for (int p = 0; p < parts; ++p) {
+        const Stats one = part(p);
+        all.s += one.s * whole_exp2(all.c - one.c);
+    }
+    return all;
 }
 
 template <typename T>
-__device__ Stats row_stats(const Row<T>& row, float k, float rest, bool with_edges, Stats* part) {
+__device__ Stats row_stats(const Row<T>& row, const Base& base, bool with_edges, Stats* part) {
     constexpr int P = Row<T>::P;
     constexpr uint32_t LOW = Pack<T>::LOW;
     Running run;
-    const float2 k2 = both(k), rest2 = both(rest);
+    const float k = base.k;
+    const float2 k2 = both(k), rest2 = both(base.rest);
+    // a vector's sum on its own: small terms added to the whole sum one by one would be lost in it
     auto take = [&](const uint4& q) {
         float2 v[P];
         Pack<T>::pairs(q, v);
         const float2 c2 = both(run.c);
         #pragma unroll
-        for (int j = 0; j < P; ++j) run.s = add2(run.s, exp2_2(fma2(v[j], rest2, fma2(v[j], k2, c2))));
+        for (int j = 0; j < P; ++j) v[j] = exp2_2(fma2(v[j], rest2, fma2(v[j], k2, c2)));
+        #pragma unroll
+        for (int j = 1; j < P; ++j) v[0] = add2(v[0], v[j]);
+        return v[0];
     };
     int i = row.lo + (int)threadIdx.x;
     for (; i + (BATCH - 1) * THREADS < row.hi; i += BATCH * THREADS) {
@@ -248,8 +272,10 @@ __device__ Stats row_stats(const Row<T>& row, float k, float rest, bool with_edg
         #pragma unroll
         for (int u = 0; u < BATCH; ++u) q[u] = row.base[i + u * THREADS];
         run.raise(Pack<T>::top(q), k);
+        float2 sum = take(q[0]);
         #pragma unroll
-        for (int u = 0; u < BATCH; ++u) take(q[u]);
+        for (int u = 1; u < BATCH; ++u) sum = add2(sum, take(q[u]));
+        run.s = add2(run.s, sum);
     }
     if (i < row.hi) {                    // the last batch, with -inf where there is no vector
         uint4 q[BATCH];
@@ -258,23 +284,17 @@ __device__ Stats row_stats(const Row<T>& row, float k, float rest, bool with_edg
             q[u] = i + u * THREADS < row.hi ? row.base[i + u * THREADS] : make_uint4(LOW, LOW, LOW, LOW);
         run.raise(Pack<T>::top(q), k);
         #pragma unroll
-        for (int u = 0; u < BATCH; ++u) if (i + u * THREADS < row.hi) take(q[u]);
+        for (int u = 0; u < BATCH; ++u) if (i + u * THREADS < row.hi) run.s = add2(run.s, take(q[u]));
     }
-    if (with_edges && (int)threadIdx.x < row.edges()) run.add(gb_up(row.x[row.edge(threadIdx.x)]), k, rest);
-    Stats mine{run.m, run.s.x + run.s.y + run.s0};
-    // the sums are of 2^(x log2(e) / T + c): what c differs from the maximum's is put right once a thread
-    if (!is_far(mine.m, k)) mine.s *= fast_exp2(fmaf(-mine.m, rest, fmaf(-mine.m, k, -run.c)));
-    float top = mine.m;
+    if (with_edges && (int)threadIdx.x < row.edges()) run.add(gb_up(row.x[row.edge(threadIdx.x)]), base);
+    float sum = run.s.x + run.s.y + run.s0, top = run.m;
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (top != -INFINITY) mine.s *= fast_exp2((mine.m - top) * k);
-    mine.s = gb_warp_sum(mine.s);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = Stats{top, mine.s};
+    const float c = offset_for(top, k);
+    sum = gb_warp_sum(sum * whole_exp2(c - run.c));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = Stats{top, c, sum};
     __syncthreads();
-    Stats all = part[0];
-    #pragma unroll
-    for (int w = 1; w < WARPS; ++w) all = merge(all, part[w], k);
-    return all;
+    return join(WARPS, k, [&](int w) { return part[w]; });
 }
 
 // The sum alone of a block's share, by differences, for a maximum that is far.
@@ -300,13 +320,14 @@ __device__ float far_sum(const Row<T>& row, float m, float k, bool with_edges, S
 // The gradient of this block's share of a row whose log-probability has the gradient `coef`;
 // zeros from vocab to ld.  `out` lies across its vectors as the row does.
 template <typename T>
-__device__ void write_grad(const Row<T>& row, T* out, int ld, int target, float coef, Stats stats, float k, float rest,
-                           float inv_temperature, bool with_edges) {
+__device__ void write_grad(const Row<T>& row, T* out, int ld, int target, float coef, Stats stats, const Base& base,
+                           bool with_edges) {
     constexpr int N = Row<T>::N, P = Row<T>::P;
-    // p = 2^(x k + c) / s with c near -m k: c's rounding, and what k leaves out at m, go into s
+    // p = 2^(x k + c) / s; what k leaves out goes into s, as it is at the maximum
+    const float k = base.k, c = stats.c, inv_temperature = (float)base.inv_temperature;
     const bool far = is_far(stats.m, k);
-    const float c = far ? 0.0f : -stats.m * k;
-    const float s = far ? stats.s : stats.s * fast_exp2(fmaf(stats.m, k, c)) * fast_exp2(-stats.m * rest);
+    const float left = far ? 0.0f : stats.m * base.rest;
+    const float s = stats.s * (fabsf(left) < 0.001f ? 1.0f - left * 0.69314718f : fast_exp2(-left));
     const float scale = -coef * inv_temperature / s, hit = coef * inv_temperature;
     const float2 k2 = both(k), c2 = both(c), scale2 = both(scale);
     uint4* to = reinterpret_cast<uint4*>(out - row.skew);
@@ -378,7 +399,7 @@ __device__ double block_sum(double v) {
 struct ForwardArgs {
     Rows rows;
     const long long* targets;
-    float inv_temperature;
+    Base base;
     float* logprobs;                     // [rows]
     float2* stats;                       // [rows] maximum and sum, or null
     // the policy loss
@@ -418,8 +439,7 @@ __global__ void __launch_bounds__(THREADS, 5) forward_kernel(const ForwardArgs a
     const int parts = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const long long r = blockIdx.x / parts;
     const bool first = rank == 0;
-    const float k = LOG2E * a.inv_temperature;
-    const float rest = fmaf(LOG2E, a.inv_temperature, -k) + LOG2E_REST * a.inv_temperature;
+    const float k = a.base.k;
     const long long at = a.rows.offset(r);
     const T* x = static_cast<const T*>(a.rows.x) + at;
     const Row<T> row(x, a.rows.vocab, rank, parts);
@@ -441,12 +461,11 @@ __global__ void __launch_bounds__(THREADS, 5) forward_kernel(const ForwardArgs a
         if (MODE == POLICY && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
-    Stats stats = row_stats(row, k, rest, first, s_part);
+    Stats stats = row_stats(row, a.base, first, s_part);
     if (parts > 1) {
         if (threadIdx.x == 0) s_block = stats;
         cluster.sync();
-        stats = *cluster.map_shared_rank(&s_block, 0);
-        for (int p = 1; p < parts; ++p) stats = merge(stats, *cluster.map_shared_rank(&s_block, p), k);
+        stats = join(parts, k, [&](int p) { return *cluster.map_shared_rank(&s_block, p); });
     }
     if (is_far(stats.m, k)) {            // the same in every block of the cluster
         stats.s = far_sum(row, stats.m, k, first, s_part);
@@ -458,7 +477,6 @@ __global__ void __launch_bounds__(THREADS, 5) forward_kernel(const ForwardArgs a
             for (int p = 0; p < parts; ++p) stats.s += cluster.map_shared_rank(&s_block, p)->s;
         }
     }
-    if (stats.s < 1.0f) stats.s = 1.0f;  // the maximum's own term is 1: what is less is rounding
     if (threadIdx.x == 0) {
         const float picked = gb_up(x[target]);
         float adv = 0.0f, old = 0.0f, ref = 0.0f;
@@ -467,7 +485,11 @@ __global__ void __launch_bounds__(THREADS, 5) forward_kernel(const ForwardArgs a
             old = a.old[r];
             if (a.ref) ref = a.ref[r];
         }
-        const float logprob = (picked - stats.m) * a.inv_temperature - logf(stats.s);
+        // in 64 bits: the numbers are some 20 and their difference may be anything
+        const double at_max = is_far(stats.m, k) ? (double)picked - (double)stats.m : (double)picked;
+        const double exact = at_max * a.base.inv_temperature + (double)stats.c * 0.69314718055994530942 -
+                             log((double)stats.s) - EXP2_LOW;
+        const float logprob = exact > 0.0 ? 0.0f : (float)exact;
         if (first) {
             a.logprobs[r] = logprob;
             if (a.stats) a.stats[r] = make_float2(stats.m, stats.s);
@@ -501,7 +523,7 @@ __global__ void __launch_bounds__(THREADS, 5) forward_kernel(const ForwardArgs a
         __syncthreads();
         const float coef = s_coef;
         if (coef == 0.0f) write_zeros(row, out, a.rows.ld, first);
-        else write_grad(row, out, a.rows.ld, (int)target, coef, stats, k, rest, a.inv_temperature, first);
+        else write_grad(row, out, a.rows.ld, (int)target, coef, stats, a.base, first);
     }
     if (parts > 1) cluster.sync();       // no block leaves while another may read its result
 }
@@ -535,7 +557,7 @@ struct GradArgs {
     const float2* stats;
     const float* coef;                   // [rows]
     const float* upstream;               // one value that multiplies every coefficient, or null
-    float inv_temperature;
+    Base base;
     void* grad;
     int parts;                           // blocks a row
 };
@@ -543,8 +565,6 @@ struct GradArgs {
 template <typename T>
 __global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
     const float up = a.upstream ? *a.upstream : 1.0f;
-    const float k = LOG2E * a.inv_temperature;
-    const float rest = fmaf(LOG2E, a.inv_temperature, -k) + LOG2E_REST * a.inv_temperature;
     const long long r = blockIdx.x / a.parts;
     const int part = (int)(blockIdx.x - r * a.parts);
     const Row<T> row(static_cast<const T*>(a.rows.x) + a.rows.offset(r), a.rows.vocab, part, a.parts);
@@ -554,7 +574,7 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(const GradArgs a) {
     if (target < 0 || target >= a.rows.vocab || own == 0.0f || coef == 0.0f) write_zeros(row, out, a.rows.ld, part == 0);
     else {
         const float2 st = a.stats[r];
-        write_grad(row, out, a.rows.ld, (int)target, coef, Stats{st.x, st.y}, k, rest, a.inv_temperature, part == 0);
+        write_grad(row, out, a.rows.ld, (int)target, coef, Stats{st.x, offset_for(st.x, a.base.k), st.y}, a.base, part == 0);
     }
 }
 
@@ -675,6 +695,11 @@ int start_forward(int dtype, const ForwardArgs& a, bool early, cudaStream_t stre
     return (int)cudaErrorInvalidValue;
 }
 
+Base base_of(double temperature) {
+    const double k = 1.4426950408889634074 / temperature;
+    return Base{(float)k, (float)(k - (double)(float)k), 1.0 / temperature};
+}
+
 bool bad(const Rows& r) {
     return r.rows <= 0 || r.inner <= 0 || r.vocab <= 0 || r.ld < r.vocab || r.ld > 0x7fffff00;
 }
@@ -687,11 +712,11 @@ bool bad(const Rows& r) {
 // without gaps, and each of its rows is as far from a 16-byte boundary as the logits' row.
 extern "C" int gb_token_logprobs(int dtype, const void* logits, long long batch_stride, long long row_stride,
                                  long long inner, long long rows, int vocab, int ld, const long long* targets,
-                                 float temperature, float* logprobs, float* stats, cudaStream_t stream) {
+                                 double temperature, float* logprobs, float* stats, cudaStream_t stream) {
     ForwardArgs a = {};
     a.rows = Rows{logits, batch_stride, row_stride, inner, rows, vocab, ld};
     if (bad(a.rows)) return (int)cudaErrorInvalidValue;
-    a.targets = targets; a.inv_temperature = 1.0f / temperature; a.logprobs = logprobs;
+    a.targets = targets; a.base = base_of(temperature); a.logprobs = logprobs;
     a.stats = reinterpret_cast<float2*>(stats);
     return start_forward<LOGPROBS>(dtype, a, false, stream);
 }
@@ -700,14 +725,14 @@ extern "C" int gb_token_logprobs(int dtype, const void* logits, long long batch_
 // null; grad null: backward is gb_logprob_grad with `coef` and `stats` (null where grad is given).
 extern "C" int gb_policy_loss(int dtype, const void* logits, long long batch_stride, long long row_stride,
                               long long inner, long long rows, int vocab, int ld, const long long* targets,
-                              float temperature, const float* old, const float* advantages, const float* ref,
+                              double temperature, const float* old, const float* advantages, const float* ref,
                               const float* weights, const float* denominator, float clip_low, float clip_high,
                               float kl_coef, float* logprobs, float* stats, float* coef, float* scratch,
                               float* loss, float* kl, float* clipped, void* grad, cudaStream_t stream) {
     ForwardArgs a = {};
     a.rows = Rows{logits, batch_stride, row_stride, inner, rows, vocab, ld};
     if (bad(a.rows)) return (int)cudaErrorInvalidValue;
-    a.targets = targets; a.inv_temperature = 1.0f / temperature; a.logprobs = logprobs;
+    a.targets = targets; a.base = base_of(temperature); a.logprobs = logprobs;
     a.stats = reinterpret_cast<float2*>(stats);
     a.old = old; a.advantages = advantages; a.ref = ref; a.weights = weights; a.denominator = denominator;
     a.clip_low = clip_low; a.clip_high = clip_high; a.kl_coef = kl_coef;
@@ -721,13 +746,13 @@ extern "C" int gb_policy_loss(int dtype, const void* logits, long long batch_str
 
 extern "C" int gb_logprob_grad(int dtype, const void* logits, long long batch_stride, long long row_stride,
                                long long inner, long long rows, int vocab, int ld, const long long* targets,
-                               float temperature, const float* stats, const float* coef, const float* upstream,
+                               double temperature, const float* stats, const float* coef, const float* upstream,
                                void* grad, cudaStream_t stream) {
     GradArgs a = {};
     a.rows = Rows{logits, batch_stride, row_stride, inner, rows, vocab, ld};
     if (bad(a.rows)) return (int)cudaErrorInvalidValue;
     a.targets = targets; a.stats = reinterpret_cast<const float2*>(stats); a.coef = coef; a.upstream = upstream;
-    a.inv_temperature = 1.0f / temperature; a.grad = grad;
+    a.base = base_of(temperature); a.grad = grad;
     a.parts = parts_for(rows, vocab, dtype == GB_F32 ? 4 : 2);
     const long long grid = rows * a.parts;
     if (dtype == GB_F32) return start(grad_kernel<float>, grid, THREADS, 1, false, stream, a);

@@ -31,15 +31,15 @@ int gb_residual_norm_bwd(int s, int u, int y, int vec, const void* d_stream, con
                          float* gate_part, void* out0, void* out1, void* out2, void* out3, void* gate_out,
                          long long rows, long long group_rows, int d, int layer, float scale, cudaStream_t cuda_stream);
 int gb_token_logprobs(int dtype, const void* logits, long long batch_stride, long long row_stride, long long inner,
-                      long long rows, int vocab, int ld, const long long* targets, float temperature, float* logprobs,
+                      long long rows, int vocab, int ld, const long long* targets, double temperature, float* logprobs,
                       float* stats, cudaStream_t stream);
 int gb_policy_loss(int dtype, const void* logits, long long batch_stride, long long row_stride, long long inner,
-                   long long rows, int vocab, int ld, const long long* targets, float temperature, const float* old,
+                   long long rows, int vocab, int ld, const long long* targets, double temperature, const float* old,
                    const float* advantages, const float* ref, const float* weights, const float* denominator,
                    float clip_low, float clip_high, float kl_coef, float* logprobs, float* stats, float* coef,
                    float* scratch, float* loss, float* kl, float* clipped, void* grad, cudaStream_t stream);
 int gb_logprob_grad(int dtype, const void* logits, long long batch_stride, long long row_stride, long long inner,
-                    long long rows, int vocab, int ld, const long long* targets, float temperature, const float* stats,
+                    long long rows, int vocab, int ld, const long long* targets, double temperature, const float* stats,
                     const float* coef, const float* upstream, void* grad, cudaStream_t stream);
 int gb_preference_loss(const float* logprobs, const long long* targets, const long long* offsets, long long rows,
                        long long length, int sequences, int vocab, int average, const void* ref, int ref_double,
@@ -321,7 +321,7 @@ Tensor logits_grad(const Tensor& logits, int64_t vocab, const Tensor& targets, d
     Tensor grad = r.grad();
     if (r.rows) {
         c10::cuda::CUDAGuard guard(grad.device());
-        check(gb_logprob_grad(GB_ROWS(r), targets_of(targets), (float)temperature, f32(stats), f32(coef), f32(upstream),
+        check(gb_logprob_grad(GB_ROWS(r), targets_of(targets), temperature, f32(stats), f32(coef), f32(upstream),
                               grad.data_ptr(), stream_of(grad)), "gb_logprob_grad", 1);
     }
     return grad;
@@ -332,7 +332,7 @@ std::tuple<Tensor, Tensor> logprobs_of(const Rows& r, const Tensor& targets, dou
     if (keep) stats = floats({r.rows, 2}, r.logits);
     if (r.rows) {
         c10::cuda::CUDAGuard guard(logprobs.device());
-        check(gb_token_logprobs(GB_ROWS(r), targets_of(targets), (float)temperature, f32(logprobs), f32(stats),
+        check(gb_token_logprobs(GB_ROWS(r), targets_of(targets), temperature, f32(logprobs), f32(stats),
                                 stream_of(logprobs)), "gb_token_logprobs", 1);
     }
     return {logprobs, stats};
@@ -389,7 +389,7 @@ PolicyResult policy_forward(const Tensor& logits, const Tensor& targets, int64_t
     const Tensor scratch = floats({4 * r.rows + 1}, logits);
     out.coef = scratch.slice(0, 3 * r.rows + 1);
     c10::cuda::CUDAGuard guard(logits.device());
-    check(gb_policy_loss(GB_ROWS(r), targets_of(targets), (float)p.temperature, f32(p.old), f32(p.advantages), f32(p.ref),
+    check(gb_policy_loss(GB_ROWS(r), targets_of(targets), p.temperature, f32(p.old), f32(p.advantages), f32(p.ref),
                          f32(p.weights), f32(p.denominator), (float)p.clip_low, (float)p.clip_high, (float)p.kl_coef,
                          f32(out.logprobs), f32(out.stats), f32(out.coef), f32(scratch), f32(out.loss), f32(out.kl),
                          f32(out.clipped), ptr(out.grad), stream_of(logits)), "gb_policy_loss", 2);
