@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(MOST) join_bwd_kernel(const JoinArgs a) {
             from_stream.fetch(lane, at, exists);
         }
         from_grad.fetch(lane, at, exists && a.d_stream);
-        if (OWN) from_update.fetch(lane, at, exists);
+        if (OWN) from_update.fetch(lane, at, exists && (a.post_weight || a.gate));
         feed_commit();
     };
     for (int i = 0; i < a.slots; ++i) fetch(i * per_slot, lo + i < hi);
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(MOST) join_bwd_kernel(const JoinArgs a) {
             #pragma unroll
             for (int e = 0; e < P; ++e) dr[e] = mul2(dr[e], both(a.scale));
         }
-        to_update.put(lane, dr, a.d);
+        if (a.d_update) to_update.put(lane, dr, a.d);
     }
     if (OWN && a.gate && gate.group >= 0) flush();
     const int sums = (NEXT ? (a.bias ? 2 : 1) : 0) + (a.post_weight ? (a.post_bias ? 2 : 1) : 0);
@@ -948,7 +948,7 @@ extern "C" void gb_residual_norm_workers(long long rows, int d, int vec, int* bl
 }
 
 // The stream, both gradients (either may be null) and the outputs are [rows, d] without gaps;
-// d_residual may be null.  out: the gradients of weight, bias, post_weight, post_bias that exist
+// d_residual and d_update may be null.  out: the gradients of weight, bias, post_weight, post_bias that exist
 // (the first two only where d_normed is given), in this order; gate_out [rows / group_rows, d].
 extern "C" int gb_residual_norm_bwd(int s, int u, int y, int vec, const void* d_stream, const void* d_normed,
                                     const void* stream, const void* update, long long update_stride,

@@ -187,8 +187,19 @@ struct ResidualNorm : Function<ResidualNorm> {
         const int64_t d = stream.size(-1);
         const Tensor u = rows_of(update, d);
         const int64_t rows = u.size(0), groups = a.groups();
-        if (ctx->saved_data["residual"].toBool()) result[0] = at::empty(stream.sizes(), stream.options());
-        result[1] = at::empty(update.sizes(), update.options());
+        // without a norm or a gate of its own the update's gradient is scale times the stream's, and
+        // without a following norm the stream's is the one that came
+        const bool own = a.post_weight.defined() || a.gate.defined();
+        const bool same = !own && a.scale == 1.0 && update.scalar_type() == stream.scalar_type();
+        const bool through = !own && !d_normed.defined();
+        if (through && (same || !rows)) {
+            result[0] = d_stream;
+            result[1] = rows ? d_stream : at::empty(update.sizes(), update.options());
+            return once(std::move(result));
+        }
+        if (through) result[0] = d_stream;
+        else if (ctx->saved_data["residual"].toBool() || same) result[0] = at::empty(stream.sizes(), stream.options());
+        result[1] = same ? result[0] : at::empty(update.sizes(), update.options());
         const Tensor* params[4] = {&a.weight, &a.bias, &a.post_weight, &a.post_bias};
         void* slots[4] = {};
         int64_t sums = 0;
@@ -214,8 +225,8 @@ struct ResidualNorm : Function<ResidualNorm> {
         check(gb_residual_norm_bwd(code_of(stream.scalar_type()), code_of(u.scalar_type()), code_of(a.out), vec,
                                    ptr(d_stream), ptr(d_normed), stream.data_ptr(), u.data_ptr(), u.stride(0),
                                    static_cast<float*>(stats.data_ptr()), ptr(a.weight), ptr(a.bias), ptr(a.post_weight),
-                                   ptr(a.post_bias), param_code, ptr(a.gate), a.gate_code(), ptr(result[0]),
-                                   result[1].data_ptr(), at, at + apart, slots[0], slots[1], slots[2], slots[3],
+                                   ptr(a.post_bias), param_code, ptr(a.gate), a.gate_code(),
+                                   through ? nullptr : ptr(result[0]), same ? nullptr : result[1].data_ptr(), at, at + apart, slots[0], slots[1], slots[2], slots[3],
                                    ptr(result[6]), rows, rows / groups, (int)d, a.layer, (float)a.scale, stream_of(stream)),
               "gb_residual_norm_bwd", 2);
         return once(std::move(result));

@@ -257,6 +257,31 @@ def test_autocast_gives_the_type_of_the_next_product():
     assert grad.dtype == torch.float32 and torch.isfinite(grad).all()
 
 
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+@pytest.mark.parametrize("stream,low", [(BF16, BF16), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("width", [100, 512])
+def test_plain_joins(scale, stream, low, width):
+    """Without a post norm or a gate; with and without the following norm's gradient."""
+    Case((3, 17, width), "rms", stream, low, F32, post=False, gate="none", scale=scale).run().check()
+    Case((3, 17, width), "layer", stream, low, F32, post=False, gate="none", scale=scale).run(d_normed=None).check()
+    Case((3, 17, width), "rms", stream, low, F32, post=False, gate="none", next=False, scale=scale).run().check()
+
+
+def test_gradients_that_are_alike_do_not_share_memory():
+    from gpubridge_b200.ops.residual_norm import residual_norm
+    r, u = (torch.randn(4, 64, device=DEV, requires_grad=True) for _ in range(2))
+    w = torch.ones(64, device=DEV)
+    for weight in (w, None):
+        r.grad = u.grad = None
+        for _ in range(2):
+            out = residual_norm(r, u, weight)
+            (out.stream.square().sum() + (out.normed.sum() if weight is not None else 0)).backward()
+        assert torch.equal(r.grad, u.grad) and r.grad.data_ptr() != u.grad.data_ptr()
+        before = u.grad.clone()
+        r.grad.zero_()
+        assert torch.equal(u.grad, before)
+
+
 def test_differences():
     """The gradients against differences of the plain form in 64 bits (CPU), and the kernel's
     gradients against those of the plain form."""
