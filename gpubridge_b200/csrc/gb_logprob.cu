@@ -24,11 +24,11 @@
 //
 // Bound by memory, but closely followed by the instructions: a value costs one exponential a sweep
 // and about four others (packed maxima, packed fused multiply-adds).  One B200, 8192 x 50257 bf16:
-// log-probabilities 137 us (6.0 TB/s), a policy step 301 us where reading and writing every counted
+// log-probabilities 137 us (6.0 TB/s), a policy step 302 us where reading and writing every counted
 // row once would take 239.  Five blocks of 256 threads an SM were better than three of 512 (323 us),
 // than six (307 us) and than rows kept in shared memory for the second sweep (376 us): what counts
 // is loads under way, and the rows in flight (74 MB) mostly stay in L2 when the gradient is stored
-// past it (344 us without that).  A preference step of 4096 x 128256 takes 448 us; its two reads and
+// past it (344 us without that).  A preference step of 4096 x 128256 takes 450 us; its two reads and
 // one write are 1.84 + 0.79 GB, 407 us.
 #include <cooperative_groups.h>
 #include <math.h>

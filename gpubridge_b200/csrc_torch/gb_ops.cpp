@@ -1,7 +1,8 @@
 // Front end in C++ of the fine-tuning operators: residual join, log-probability losses, gradient
 // norm and clipped AdamW.  The kernels are those of the native library; here are their autograd
 // nodes and the memory they need, so that a call costs microseconds of host time (a forward and
-// backward pass of the residual join through Python functions: 200 us, through these: 40 us).
+// backward pass of the residual join through Python functions: 208 us; through these 95 us, of which
+// torch's autograd engine takes some 65).
 //
 // Arguments are checked in Python (gpubridge_b200/ops); an entry point here only answers None where
 // they are not what the kernels take, and Python then says why.
