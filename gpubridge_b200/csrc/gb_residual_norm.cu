@@ -23,7 +23,7 @@
 //   8192 x 768, layer norm, fp32 stream and bf16 update     22 / 26 us   (75 / 113 MB: 12 / 18 us)
 //   8192 x 2048, bf16, both norms and a gate                 29 / 43 us   (134 / 201 MB: 21 / 31 us)
 //   4096 x 4096, bf16, both norms and sequence gates         31 / 55 us   (the same bytes)
-//   3333 x 1001, fp32, post norm and sequence gates          16 / 25 us   (40 / 53 MB: 6 / 8 us)
+//   3333 x 1001, fp32, post norm and sequence gates          18 / 25 us   (40 / 53 MB: 6 / 8 us)
 // What it took at 8192 x 2048: loads in registers and one barrier after another 186 us; rows staged
 // ahead 132; packed arithmetic and two rows at a time 99; 16 columns a thread instead, with copies
 // that need no branch, 94; parameters in shared memory instead of spilled registers 77; sums of one
