@@ -201,8 +201,10 @@ struct Row {
     __device__ __forceinline__ int edge(int i) const { return i < head ? i : tail + i - head; }
 };
 
-// Where x k leaves fp32: a row whose maximum is the type's lowest value (all of it masked), or inf.
-__device__ __forceinline__ bool is_far(float m, float k) { return !(fabsf(m) * k < 1e38f); }
+// From 2^30 on the product m k is rounded by more than 32, and terms could leave fp32's range: a row
+// whose maximum is a mask's -1e9, the type's lowest value, or inf.  Neighbours there are 2^-64 of one
+// another, so that a far running maximum may drop its terms once a nearer one is found.
+__device__ __forceinline__ bool is_far(float m, float k) { return !(fabsf(m) * k < 1073741824.0f); }
 
 // A row's terms are 2^(x k + c) with c the whole number next to -m k, m the row's maximum: sums of
 // different c are joined by powers of two, without a rounding.

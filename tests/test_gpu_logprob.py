@@ -130,6 +130,29 @@ def test_masked_columns_infinities_and_nan():
         assert (grad[[3, 4, 5]] == 0).all()
 
 
+@pytest.mark.parametrize("level", [-1e9, 1e7, -3e8, -744261120.0, 1e10, -1e20, 1e30])
+def test_rows_far_from_zero(level):
+    """All columns at a mask's value or beyond, some around 2^30 / log2(e).  From 1e8 on neighbours are
+    so far apart that only ties share a row's weight; below 2^30 an exponent is then off by the roundings
+    of numbers of up to 96 (2^-18 twice, 2^-19) and of 2^30 times log2(e)'s 2^-48: 1.4e-5, less than
+    600 H.  At 1e7, in steps of 2.4, what a probability of 2^-87 misses is 87 * 2^-24 of itself."""
+    from gpubridge_b200.ops.logprob import token_logprobs
+    logits, g = _logits((6, 3001), F32, seed=15)
+    step = abs(level) * 2.0 ** -22
+    logits = (level + torch.round(logits.double() * 2) * step).float()
+    logits[1, ::2] = 0.5 * level                            # half the columns elsewhere
+    logits[2, 5:] = -math.inf
+    targets = torch.randint(3001, (6,), device=DEV, generator=g)
+    targets[2] = 3
+    leaf = logits.requires_grad_(True)
+    got = token_logprobs(leaf, targets)
+    want, p, counted = _wide(logits, targets, 3001)
+    assert ((got - want).abs() <= LOGPROB_TOL + 64 * H * want.abs()).all(), (got, want)
+    grad, = torch.autograd.grad(got.sum(), leaf)
+    off = (grad.double() + p - torch.nn.functional.one_hot(targets, 3001)).abs()
+    assert (off <= 600 * H * p + 4 * H + 1e-37).all()
+
+
 def test_large_logits_and_a_dominant_target():
     from gpubridge_b200.ops.logprob import token_logprobs
     logits, g = _logits((6, 5000), F32, seed=6, std=5.0)
