@@ -43,8 +43,8 @@ struct JoinArgs {
     const void *weight, *bias, *post_weight, *post_bias, *gate;     // null where absent
     const void *d_stream, *d_normed;   // [rows, d] or null
     void *d_residual, *d_update;
-    float* part;                       // [workers][sums][d]
-    float* gate_part;                  // [workers + groups - 1][d]
+    float* part;                       // [blocks][sums][d]
+    float* gate_part;                  // [owners + groups - 1][d]
     long long rows, group_rows;        // rows of one gate group
     int d, layer, param_code, gate_code, next, slots;
     int owners;                        // teams that have rows, at least one each
@@ -52,7 +52,7 @@ struct JoinArgs {
 };
 
 constexpr int MAX_THREADS = 512;
-constexpr int REDUCER_FLOATS = 2 * 2 * (MAX_THREADS / 32) * 4;   // three warps a team take the room of four
+constexpr int REDUCER_FLOATS = 2 * 2 * (MAX_THREADS / 32) * 4;   // two to four warps a team take the room of four
 
 // A block is blockDim.y teams of blockDim.x threads; a team owns a row.  An SM holds one block, so
 // that a backward pass leaves one row of partial sums for each SM.
@@ -81,8 +81,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // Sums of Q values over a team's threads, one barrier a reduction: the buffers alternate.  Within
-// a warp the values are exchanged for one another before they are added, so that Q = 1, 2, 4 cost
-// five, five and six shuffles.
+// a warp two values are exchanged for one another before they are added: five shuffles for either.
 struct Reducer {
     float* buffer;                     // [2][warps, to a multiple of four][4]
     int warps, half, parity;
@@ -97,26 +96,16 @@ struct Reducer {
     }
     template <int Q>
     __device__ void sum(float (&v)[Q]) {
-        static_assert(Q == 1 || Q == 2 || Q == 4, "values of one reduction");
+        static_assert(Q == 1 || Q == 2, "values of one reduction");
         const int lane = threadIdx.x & 31;
-        float mine;
-        if constexpr (Q == 4) {
-            const bool upper = lane & 16;
-            float a = upper ? v[2] : v[0], b = upper ? v[3] : v[1];
-            const float sa = upper ? v[0] : v[2], sb = upper ? v[1] : v[3];
-            a += __shfl_xor_sync(0xffffffffu, sa, 16);
-            b += __shfl_xor_sync(0xffffffffu, sb, 16);
-            const bool second = lane & 8;
-            mine = second ? b : a;
-            mine += __shfl_xor_sync(0xffffffffu, second ? a : b, 8);
-        } else if constexpr (Q == 2) {
+        float mine = v[0];
+        if constexpr (Q == 2) {
             const bool upper = lane & 16;
             mine = upper ? v[1] : v[0];
             mine += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[1], 16);
-        } else mine = v[0];
+        }
         #pragma unroll
-        for (int step = Q == 4 ? 4 : Q == 2 ? 8 : 16; step > 0; step >>= 1)
-            mine += __shfl_xor_sync(0xffffffffu, mine, step);
+        for (int step = Q == 2 ? 8 : 16; step > 0; step >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, step);
         if (warps == 1) {
             #pragma unroll
             for (int q = 0; q < Q; ++q) v[q] = Q == 1 ? mine : __shfl_sync(0xffffffffu, mine, q * (32 / Q));
